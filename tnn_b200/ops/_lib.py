@@ -154,6 +154,22 @@ def raw_stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *_):
+        return False
+
+
+_HERE = _Here()
+
+
+def device_of(t):
+    """Context in which ``t``'s device is the current one: what is launched goes to that device, on its current stream."""
+    return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
 def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
@@ -195,7 +211,7 @@ def check_status(device=None):
         raise RuntimeError(f"tnn_b200 kernel reported status {code}: {_STATUS_NAMES.get(code, '?')}")
 
 
-_BOUNDS_FILES = ("elementwise", "loss_optim", "conv_pool", "batchnorm")
+_BOUNDS_FILES = ("elementwise", "loss_optim", "conv_pool", "batchnorm", "embedding", "token_logprob")
 
 
 def fetch_bounds_violations():

@@ -11,6 +11,8 @@ them runs anywhere.
     h, s = F.add_layer_norm(x, delta, g, b)     # s = x + delta ; h = LN(s)
     o = F.causal_self_attention(qkv, heads)     # qkv [B, S, 3E] packed q | k | v
     l = F.cross_entropy(logits, labels)         # mean over rows
+    e = F.embedding(ids, table, scale)          # rows of a token table; the table's gradient is summed per token in a fixed order
+    t = F.token_log_probs(logits, tokens, 5)    # log probability per token, entropy, top alternatives
 
 Gradients with respect to parameters are accumulated in fp32 and rounded once to the parameter's dtype, by autograd or, for
 the weights of few rows, where they are computed.
@@ -177,3 +179,53 @@ def cross_entropy(logits: torch.Tensor, labels: torch.Tensor, return_corrects: b
     ``return_corrects`` also the number of rows whose arg-max equals the label (computed by the same kernel)."""
     loss, corrects = _CrossEntropy.apply(logits, labels)
     return (loss, corrects) if return_corrects else loss
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.args = (table.shape[0], scale, padding_idx)
+        return raw.embedding_lookup(ids, table, scale, padding_idx)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        rows, scale, padding_idx = ctx.args
+        return None, raw.embedding_grad(ids, dy, rows, scale, padding_idx), None, None
+
+
+def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * table[ids]`` (zeros at ``padding_idx``), shape ``[*ids.shape, width]``. The table's gradient adds each token's
+    positions up in fp32, in an order that depends on the ids alone, and rounds once to the table's type."""
+    return _Embedding.apply(ids, table, float(scale), padding_idx)
+
+
+class _TokenLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
+        keep = {}
+        r = raw.token_log_probs(logits, tokens, top_k, temperature, ignore_index, keep)
+        ctx.save_for_backward(logits, tokens, keep["stats"], keep["entropy"])
+        ctx.args = (temperature, ignore_index)
+        ctx.mark_non_differentiable(r.top_log_probs, r.top_indices)
+        ctx.set_materialize_grads(False)
+        return tuple(r)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, h, *_):
+        logits, tokens, stats, entropy = ctx.saved_tensors
+        if g is None and h is None:
+            return None, None, None, None, None
+        return raw.token_log_probs_grad(logits, tokens, {"stats": stats, "entropy": entropy}, g, h, *ctx.args), None, None, None, None
+
+
+def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, temperature: float = 1.0,
+                    ignore_index: int = -100) -> raw.TokenLogProbs:
+    """:func:`raw.token_log_probs` with gradients through the log probabilities and the entropies (the alternatives are
+    reported, not differentiated): one pass over the logits forward, one read and one write backward."""
+    if not (logits.requires_grad and torch.is_grad_enabled()):
+        return raw.token_log_probs(logits, tokens, top_k, temperature, ignore_index)
+    return raw.TokenLogProbs(*_TokenLogProbs.apply(logits, tokens, top_k, float(temperature), int(ignore_index)))
