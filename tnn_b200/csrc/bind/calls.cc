@@ -75,7 +75,7 @@ const Entry SIGNATURES[] = {
     SIG("ppppliillfupp"),                               // embedding_fwd, embedding_bwd
     SIG("piplplillfip"), SIG("piplppppp" "iillfiiiip"),  // embed_lookup, embed_grad
     SIG("plpipppppliiflip"), SIG("plplpipppp" "liffl" "ip"),  // token_logprob, token_logprob_grad
-    SIG("plliiiipif" "ppppppppp"),  // newton_schulz
+    SIG("plliiiipif" "pppppppppp"),  // newton_schulz
     SIG("plplip"), SIG("pplp"), SIG("plpplip"),         // colsum_accum, cast_f32_bf16, scale_by
     SIG("pppppppp" "liffupp"),                          // layernorm_fwd
     SIG("pppppppppp" "lifupp"), SIG("ppppppppppp" "lifupp"),  // layernorm_bwd, layernorm_bwd_db

@@ -1475,9 +1475,8 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-int encode_tmap_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
-                     const uint64_t* strides_bytes, const uint32_t* box,
-                     const uint32_t* elem_strides) {
+static int encode_tmap_16bit(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                             const uint32_t* box, const uint32_t* elem_strides, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return -1;
   cuuint64_t gdim[5];
@@ -1491,9 +1490,17 @@ int encode_tmap_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t*
     if (i > 0) gstr[i - 1] = strides_bytes[i - 1];
   }
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim, gstr,
-                  bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -static_cast<int>(r) - 100;
+}
+int encode_tmap_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                     const uint32_t* elem_strides) {
+  return encode_tmap_16bit(m, base, rank, dims, strides_bytes, box, elem_strides, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int encode_tmap_bf16_sw64(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                          const uint32_t* box) {
+  return encode_tmap_16bit(m, base, rank, dims, strides_bytes, box, nullptr, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // Same as encode_tmap_bf16 for fp32 elements (128-byte swizzle: the inner box extent is at most 32 elements).

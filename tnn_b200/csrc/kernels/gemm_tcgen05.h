@@ -25,6 +25,9 @@ enum GemmEpilogue : int {
 int encode_tmap_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
                      const uint64_t* strides_bytes, const uint32_t* box,
                      const uint32_t* elem_strides);
+// The same with 64-byte swizzle (the inner box extent is at most 32 elements).
+int encode_tmap_bf16_sw64(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                          const uint32_t* box);
 int encode_tmap_f32(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
                     const uint32_t* box);
 int sm_count();

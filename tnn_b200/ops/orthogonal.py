@@ -21,7 +21,7 @@ def _library():
     lib = _lib.load()
     if not _DECLARED:
         p, i, l, f = _lib.c_void_p, _lib.c_int, _lib.c_ll, _lib.c_float
-        _lib.declare(lib, "tnnb_newton_schulz", [p, l, l, i, i, i, i, p, i, f, p, p, p, p, p, p, p, p, p])
+        _lib.declare(lib, "tnnb_newton_schulz", [p, l, l, i, i, i, i, p, i, f, p, p, p, p, p, p, p, p, p, p])
         _DECLARED = True
     return lib
 
@@ -47,7 +47,7 @@ def _largest(poly: Sequence[float], upto: float) -> float:
 @functools.lru_cache(maxsize=64)
 def _checked(coefficients: Tuple[float, ...]) -> object:
     """The coefficients as a C array, after a look at what they make of singular values in [0, 1]: the kernels keep X and X X^T
-    times 2^12 and b A + c A A times 2^11 in fp16, whose largest number is 65504."""
+    times 2^12 and a + b A + c A A times 2^11 in fp16, whose largest number is 65504."""
     import ctypes
 
     upto = 1.0
@@ -57,9 +57,9 @@ def _checked(coefficients: Tuple[float, ...]) -> object:
             raise ValueError(f"Newton-Schulz coefficients {(a, b, c)}")
         poly = _largest((2, b, c), upto)
         upto = 1.01 * _largest((1, a, b, c), upto)  # with room for what is rounded
-        if poly > 30 or upto > 3.9:
+        if abs(a) + poly > 30 or upto > 3.9:
             raise ValueError(f"Newton-Schulz coefficients {(a, b, c)} take singular values of [0, 1] to {upto:.3g} "
-                             f"(factor of the products {poly:.3g}): at most 3.9 (30) are supported")
+                             f"(factors of the products up to {abs(a) + poly:.3g}): at most 3.9 (30) are supported")
     return (ctypes.c_float * len(coefficients))(*coefficients)
 
 
@@ -70,7 +70,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence = QUIN
     steps or a triple for each.
 
     The result is bf16, packed, rounded once from fp32; the products take fp16 operands that are scaled into its range, X itself
-    is carried with 22 bits. A matrix of zeros stays one; NaN or infinity anywhere in a matrix make NaNs of it."""
+    is carried with 22 bits up to the last two. A matrix of zeros stays one; NaN or infinity anywhere in a matrix make NaNs of it."""
     if g.dim() < 2 or not g.is_floating_point():
         raise ValueError(f"newton_schulz takes floating-point matrices, not {tuple(g.shape)} of {g.dtype}")
     steps = int(steps)
@@ -111,14 +111,14 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence = QUIN
         most = 4096  # matrices per call
         for i in range(0, count, most):
             k = min(most, count - i)
-            parts = [(k * s + 255) // 256 * 256 for s in (size_x, size_x, size_x, size_s, size_s, 512)]
+            parts = [(k * s + 255) // 256 * 256 for s in (size_x, size_x, size_x, size_s, size_s, 512, 12 * steps + 4)]
             work = torch.empty(sum(parts), dtype=torch.uint8, device=g.device)
-            at = [work.data_ptr() + sum(parts[:j]) for j in range(6)]
+            at = [work.data_ptr() + sum(parts[:j]) for j in range(7)]
             rc = _library().tnnb_newton_schulz(x.data_ptr() + i * item * x.element_size(), item, ld, code, k, m, n, _address(c_array), steps,
                                                float(eps), out.data_ptr() + i * m * n * 2, *at, _lib.status_addr(g.device),
                                                _lib.raw_stream())
             _lib.check_rc(rc, "newton_schulz")
-            LAUNCHES["count"] += 2 + 3 * steps
+            LAUNCHES["count"] += 3
     return out
 
 
