@@ -32,6 +32,7 @@ namespace tnnb {
 
 static constexpr float NS_X = 4096.f, NS_A = 4096.f, NS_B = 2048.f;  // stored = value times this
 static constexpr int NS_EPI_WARPS = 8;
+static constexpr int NS_THREADS = 96 + 32 * NS_EPI_WARPS;
 static constexpr int NS_MAX_STEPS = 64;
 static constexpr int NS_FOLDED = 2;      // last steps in which B holds a
 
@@ -67,6 +68,13 @@ struct NsParams {
 // A tile of work.
 struct NsTask {
   int step, phase, item, mb, nb;
+};
+// Tiles on their way through a CTA, found and looked up (their inputs are complete) by a warp of its own: the divisions and the look
+// at the counter took 1.5 us between two tiles' copies.
+static constexpr int NS_RING = 4;
+struct NsRing {
+  NsTask task[NS_RING];
+  uint64_t full[NS_RING], empty[NS_RING];
 };
 
 // A product's tiles in their order. RATIO column blocks are as wide as a row block is high.
@@ -309,7 +317,7 @@ struct NsCfg {
   static constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * 128;  // this CTA's rows of B
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = BN == 64 ? 6 : 5;
-  static constexpr int SMEM = STAGES * STAGE + NS_EPI_WARPS * NS_SLOTS * NS_SLOT + 512 + 1024;
+  static constexpr int SMEM = STAGES * STAGE + NS_EPI_WARPS * NS_SLOTS * NS_SLOT + 512 + 1024;  // (and the ring)
 };
 
 struct NsMaps {
@@ -318,11 +326,11 @@ struct NsMaps {
 };
 
 // PAIR: 256 x 256 tiles over two SMs, each with 128 rows of either operand; else 128 x 128 or 128 x 64 tiles. Persistent; warp 0 copies,
-// warp 1 issues the products (two accumulators), warps 2 to 9 are the epilogue. Tile i of the whole computation belongs to worker
+// warp 1 issues the products (two accumulators), warps 2 to 9 are the epilogue, warp 10 finds the tiles. Tile i of the whole computation belongs to worker
 // i modulo their number, and a tile reads what tiles before it in this order have written: as all workers run at the same time
 // (cooperative launch), the first unfinished tile can always be worked on.
 template <int PAIR, int BN, int TALL>
-__global__ void __launch_bounds__(64 + 32 * NS_EPI_WARPS, 1)
+__global__ void __launch_bounds__(NS_THREADS, 1)
 ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsParams p) {
   using Cfg = NsCfg<PAIR, BN>;
   constexpr int TM = Cfg::TM, STAGES = Cfg::STAGES, RATIO = Cfg::RATIO;
@@ -337,6 +345,7 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
   uint64_t* slot_bars = tempty + 2;  // [epilogue warps][slots]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(slot_bars + NS_EPI_WARPS * NS_SLOTS);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  __shared__ NsRing ring;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
@@ -354,6 +363,10 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
       mbar_init(&tempty[a], PER_TILE);
     }
     for (int i = 0; i < NS_EPI_WARPS * NS_SLOTS; ++i) mbar_init(&slot_bars[i], 1);
+    for (int i = 0; i < NS_RING; ++i) {
+      mbar_init(&ring.full[i], 1);
+      mbar_init(&ring.empty[i], NS_EPI_WARPS + (rank == 0 ? 2 : 1));
+    }
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -372,24 +385,34 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  // The worker's tile number i, once its inputs are complete; next_task(i) ... gave_back(i).
+  auto next_task = [&](int i, NsTask& t) {
+    bool there = wait_or_abort(&ring.full[i % NS_RING], (i / NS_RING) & 1, abort_flag);
+    if (!there && !*abort_flag) there = wait_or_abort(&ring.full[i % NS_RING], (i / NS_RING) & 1, abort_flag);
+    if (there) t = ring.task[i % NS_RING];
+    return there;
+  };
+  const int mine = (int)((total - worker + workers - 1) / workers);  // tiles of this worker (no fewer than one: the host's grid)
+
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0, last_stage = -1;
       uint32_t phase = 0, last_phase = 0;
       bool ok = true;
-      for (long long work = worker; ok && work < total; work += workers) {
-        const NsTask t = ns_task<RATIO>(p, work);
+      for (int i = 0; ok && i < mine; ++i) {
+        NsTask t;
+        if (!next_task(i, t)) {
+          ns_give_up(p, abort_flag, ST_TIMEOUT_PRODUCER);
+          ok = false;
+          break;
+        }
+        mbar_arrive(&ring.empty[i % NS_RING]);
         const int x = t.step & 1;
         const CUtensorMap* ma = t.phase == NS_POLY ? &maps.gram : t.phase == NS_STEP && !TALL ? &maps.poly : &maps.x[x];
         const CUtensorMap* mb = t.phase == NS_POLY ? &maps.gram : t.phase == NS_STEP && TALL ? &maps.poly : &maps.x[x];
         const bool a_mn = TALL && t.phase == NS_GRAM, b_mn = t.phase == NS_GRAM ? TALL : (t.phase == NS_STEP && !TALL);
         const int row0 = t.mb * TM + rank * 128, col0 = t.nb * BN + rank * (BN / 2);  // this CTA's rows of A and of B
         const int k_blocks = t.phase == NS_GRAM ? p.k_gram : p.k_rest;
-        if (!ns_ready(p, t, PER_TILE, abort_flag)) {
-          ns_give_up(p, abort_flag, ST_TIMEOUT_PRODUCER);
-          ok = false;
-          break;
-        }
         fence_proxy_async_all();  // what other SMs have stored is visible to the copies that follow
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!wait_or_abort(&empty[stage], phase ^ 1, abort_flag)) {
@@ -445,8 +468,13 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (long long work = worker; ok && work < total; work += workers) {
-        const NsTask t = ns_task<RATIO>(p, work);
+      for (int i = 0; ok && i < mine; ++i) {
+        NsTask t;
+        if (!next_task(i, t)) {
+          ns_give_up(p, abort_flag, ST_TIMEOUT_MMA);
+          break;
+        }
+        mbar_arrive(&ring.empty[i % NS_RING]);
         const int a_mn = TALL && t.phase == NS_GRAM, b_mn = t.phase == NS_GRAM ? TALL : (t.phase == NS_STEP && !TALL);
         const uint32_t idesc = make_idesc_f16(TM, BN, a_mn, b_mn);
         const int k_blocks = t.phase == NS_GRAM ? p.k_gram : p.k_rest;
@@ -491,6 +519,18 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
         if (acc == 0) acc_phase ^= 1;
       }
     }
+  } else if (warp == 2 + NS_EPI_WARPS) {
+    if (lane == 0) {
+      for (int i = 0; i < mine; ++i) {
+        const NsTask t = ns_task<RATIO>(p, worker + (long long)i * workers);
+        if (!ns_ready(p, t, PER_TILE, abort_flag) || !wait_or_abort(&ring.empty[i % NS_RING], ((i / NS_RING) & 1) ^ 1, abort_flag)) {
+          ns_give_up(p, abort_flag, ST_TIMEOUT_PRODUCER);
+          break;
+        }
+        ring.task[i % NS_RING] = t;
+        mbar_arrive(&ring.full[i % NS_RING]);
+      }
+    }
   } else {
     const int q = warp & 3;  // TMEM lane quarter this warp may read
     constexpr int WCOLS = BN / 2;
@@ -500,17 +540,18 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (long long work = worker; work < total; work += workers) {
-      const NsTask t = ns_task<RATIO>(p, work);
+    for (int i = 0; i < mine; ++i) {
+      NsTask t;
+      ok = __all_sync(0xffffffffu, next_task(i, t));
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&ring.empty[i % NS_RING]);
+        fence_proxy_async_all();  // as in front of the operands' copies, for the addend's
+      }
       const int x = t.step & 1;
       const bool folded = t.step + NS_FOLDED >= p.steps, last = t.step + 1 == p.steps;
       const float a = p.coef[3 * t.step], b = p.coef[3 * t.step + 1], c = p.coef[3 * t.step + 2];
-      // the addend's product is complete before this warp asks for it
-      if (t.phase == NS_POLY || (t.phase == NS_STEP && !folded)) {
-        ok = __all_sync(0xffffffffu, lane != 0 || ns_ready(p, t, PER_TILE, abort_flag));
-        if (!ok) break;
-        if (lane == 0) fence_proxy_async_all();
-      }
       const int row0 = t.mb * TM + rank * 128 + q * 32, col0 = t.nb * BN + wcol;
       const bool mirror = t.nb >= RATIO * (t.mb + 1);
       const uint32_t t_addr = tmem_base + acc * BN + (static_cast<uint32_t>(q * 32) << 16) + wcol;
@@ -727,7 +768,7 @@ static cudaError_t ns_launch(const NsMaps& maps, NsParams p, cudaStream_t st) {
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = 2;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(64 + 32 * NS_EPI_WARPS);
+  cfg.blockDim = dim3(NS_THREADS);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = st;
   cfg.attrs = attr;
