@@ -53,16 +53,40 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// A vector's largest value, and its elements as pairs of fp32 that -inf has left (0 * -inf would be NaN): at least LP_LOWEST, whose
+// probability beside any logit that huge() lets pass is 0 as well. fp16 cannot hold that bound and is raised to it afterwards.
+static constexpr float LP_LOWEST = -1e20f;
 __device__ __forceinline__ float vec_max(const Vec<float, 4>& v) { return max_nan(max_nan(v.v[0], v.v[1]), max_nan(v.v[2], v.v[3])); }
+__device__ __forceinline__ void vec_pairs(const Vec<float, 4>& v, uint64_t (&x)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) x[i] = pack_f2(fmaxf(v.v[2 * i], LP_LOWEST), fmaxf(v.v[2 * i + 1], LP_LOWEST));
+}
 __device__ __forceinline__ float vec_max(const Vec<__nv_bfloat16, 8>& v) {
   const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(v.v);
   const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
   return max_nan(__low2float(m), __high2float(m));
 }
+__device__ __forceinline__ void vec_pairs(const Vec<__nv_bfloat16, 8>& v, uint64_t (&x)[4]) {
+  const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(v.v);
+  const __nv_bfloat162 lowest = __float2bfloat162_rn(LP_LOWEST);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 m = __hmax2(w[i], lowest);
+    x[i] = bf16x2_to_f2(*reinterpret_cast<const uint32_t*>(&m));
+  }
+}
 __device__ __forceinline__ float vec_max(const Vec<__half, 8>& v) {
   const __half2* w = reinterpret_cast<const __half2*>(v.v);
   const __half2 m = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
   return max_nan(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ void vec_pairs(const Vec<__half, 8>& v, uint64_t (&x)[4]) {
+  const __half2* w = reinterpret_cast<const __half2*>(v.v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(w[i]);
+    x[i] = pack_f2(fmaxf(f.x, LP_LOWEST), fmaxf(f.y, LP_LOWEST));
+  }
 }
 
 // Order of logits as unsigned integers (0: none at all), NaN above +inf, -0 equal to +0.
@@ -77,11 +101,8 @@ __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float
 // Logits from here on might overflow when they are multiplied by c. Numbers of that size differ by far more than any exponent, so
 // that (z - m) c, which loses the digits below theirs, is as good there; elsewhere z c - m c, one fused operation, is better: the
 // rounding of m c is common to all terms of a row.
-__device__ __forceinline__ bool huge(float m) { return !(fabsf(m) < 1e30f); }
-__device__ __forceinline__ float exponent(float z, float m, float c) {
-  return huge(m) ? (z - m) * c : fmaf(z, c, -__fmul_rn(m, c));
-}
-// The same between two maxima, 0 for equal ones.
+__device__ __forceinline__ bool huge(float m) { return !(fabsf(m) < 1e20f); }
+// The exponent of one maximum relative to another, 0 for equal ones.
 __device__ __forceinline__ float rescale(float m, float to, float c) {
   const float d = huge(m) || huge(to) ? (m - to) * c : __fmul_rn(m, c) - __fmul_rn(to, c);
   return fmaxf(d, LP_FLOOR);
@@ -186,35 +207,38 @@ __device__ __forceinline__ void add_candidate(LogprobShared& sh, uint32_t key, i
   if (at < LP_CAND) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~index;
 }
 
-// More elements reach the bound than there is room for: find the k-th largest key by bisection, take what lies above it
-// (fewer than k elements) and fill up with the first elements equal to it. Returns the number of candidates, k.
+// The elements with keys >= `from` among those of the listed threads become candidates. Returns their number (of which LP_CAND at most
+// are kept). Block-wide.
 template <typename T>
-__device__ int select_by_bisection(const RowReader<T>& r, int k, uint32_t bound, LogprobShared& sh) {
+__device__ int collect(const RowReader<T>& r, uint32_t from, LogprobShared& sh) {
   constexpr int PER = 16 / sizeof(T);
-  uint32_t lo = bound, hi = 0xffffffffu;  // at least k keys are >= lo; the answer lies in [lo, hi]
-  if (count_from(r, lo + 1, sh) < k) hi = lo;  // one value fills the rest, the usual reason (lo is not the largest key: keys that large are few)
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2 + 1;
-    if (count_from(r, mid, sh) >= k) lo = mid;
-    else hi = mid - 1;
-  }
-  if (threadIdx.x == 0) sh.found = 0;
-  __syncthreads();
-  for (int v = r.p.v_lo + (int)threadIdx.x; v < r.p.v_hi; v += LP_THREADS) {
-    const Vec<T, PER> w = r.vec(v);
+  const int each = (r.p.v_hi - r.p.v_lo + LP_THREADS - 1) / LP_THREADS + 1;  // a thread's vectors and its loose element
+  for (int it = threadIdx.x; it < sh.winners * each; it += LP_THREADS) {
+    const int w = sh.winner[it / each], q = it % each;
+    if (q < each - 1) {
+      const int v = r.p.v_lo + w + q * LP_THREADS;
+      if (v >= r.p.v_hi) continue;
+      const Vec<T, PER> x = r.vec(v);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const uint32_t key = key_of(to_f32(w.v[j]));
-      if (key > lo) add_candidate(sh, key, r.p.head + v * PER + j);
+      for (int j = 0; j < PER; ++j) {
+        const uint32_t key = key_of(to_f32(x.v[j]));
+        if (key >= from) add_candidate(sh, key, r.p.head + v * PER + j);
+      }
+    } else {
+      const int i = loose<T>(r.p, w);
+      if (i >= 0 && key_of(r.one(i)) >= from) add_candidate(sh, key_of(r.one(i)), i);
     }
   }
-  const int i = loose<T>(r.p, threadIdx.x);
-  if (i >= 0 && key_of(r.one(i)) > lo) add_candidate(sh, key_of(r.one(i)), i);
   __syncthreads();
-  int have = sh.found;
+  return sh.found;
+}
+
+// Fill up to k candidates with the first elements whose key is `key`; `have` candidates are there.
+template <typename T>
+__device__ int fill_equal(const RowReader<T>& r, int have, int k, uint32_t key, LogprobShared& sh) {
   for (int i0 = r.p.lo; i0 < r.p.hi && have < k; i0 += LP_THREADS) {
     const int e = i0 + threadIdx.x;
-    const bool is = e < r.p.hi && key_of(r.one(e)) == lo;
+    const bool is = e < r.p.hi && key_of(r.one(e)) == key;
     const unsigned who = __ballot_sync(0xffffffffu, is);
     if ((threadIdx.x & 31) == 0) sh.warp_count[threadIdx.x >> 5] = __popc(who);
     __syncthreads();
@@ -223,11 +247,46 @@ __device__ int select_by_bisection(const RowReader<T>& r, int k, uint32_t bound,
       if (w < (int)(threadIdx.x >> 5)) at += sh.warp_count[w];
       all += sh.warp_count[w];
     }
-    if (is && at < k) sh.cand[at] = ((unsigned long long)lo << 32) | (uint32_t)~e;
+    if (is && at < k) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~e;
     __syncthreads();
     have = min(all, k);
   }
   return have;
+}
+
+// Candidates for the k largest elements: those that reach the bound. Where many may equal it (all ruled out, all alike), those
+// above it and then the first that equal it; where more lie above it than there is room for (logits in an order that puts the largest
+// into few threads' hands), the k-th largest key is found by bisection over its bits. Returns their number, k or more.
+template <typename T>
+__device__ int select_candidates(const RowReader<T>& r, int k, uint32_t own_key, LogprobShared& sh) {
+  constexpr uint32_t RULED_OUT = 0x007fffffu;  // the key of -inf
+  constexpr int MANY = 96;                     // threads; a bound that is not shared by many is reached by about k
+  uint32_t bound = sh.bound;
+  if (own_key >= bound && own_key != 0) sh.winner[atomicAdd(&sh.winners, 1)] = threadIdx.x;
+  __syncthreads();
+  if (bound != RULED_OUT && sh.winners <= MANY) {
+    const int n = collect(r, bound, sh);
+    if (n <= LP_CAND) return n;
+  }
+  auto above = [&](uint32_t key, bool mine) {  // candidates above `key`
+    __syncthreads();
+    if (threadIdx.x == 0) sh.winners = sh.found = 0;
+    __syncthreads();
+    if (mine) sh.winner[atomicAdd(&sh.winners, 1)] = threadIdx.x;
+    __syncthreads();
+    return key == 0xffffffffu ? 0 : collect(r, key + 1, sh);
+  };
+  int n = above(bound, own_key > bound);
+  if (n > LP_CAND) {
+    uint32_t hi = 0xffffffffu;  // at least k keys are >= bound; the k-th lies in [bound, hi]
+    while (bound < hi) {
+      const uint32_t mid = bound + (hi - bound) / 2 + 1;
+      if (count_from(r, mid, sh) >= k) bound = mid;
+      else hi = mid - 1;
+    }
+    n = above(bound, own_key > bound);  // fewer than k
+  }
+  return n >= k ? n : fill_equal(r, n, k, bound, sh);
 }
 
 // The `k` largest of n candidates into best[], in order (distinct keys: a place is the number of larger ones).
@@ -240,9 +299,40 @@ __device__ __forceinline__ void rank_candidates(const unsigned long long* cand, 
   }
 }
 
+// A row's results (one warp).
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobParams& a, const Sums& all, const unsigned long long* best, long long row, const T* z) {
+  const int lane = threadIdx.x & 31;
+  const bool dead = all.m == -INFINITY, bad = !(all.m < INFINITY);  // NaN or +inf among the logits
+  const double ls = log2((double)all.s);
+  const double ln2 = 0.69314718055994530942;
+  auto log_prob = [&](float v) -> float {
+    if (bad) return NAN;
+    if (dead || v == -INFINITY) return -INFINITY;
+    const double d = huge(all.m) ? ((double)v - all.m) * a.c : (double)v * a.c - __fmul_rn(all.m, a.c);
+    return (float)((d - ls) * ln2);
+  };
+  if (lane < a.top) {
+    const unsigned long long b = best[lane];
+    a.top_logp[row * a.top + lane] = log_prob(value_of((uint32_t)(b >> 32)));
+    a.top_index[row * a.top + lane] = (long long)(uint32_t)~(uint32_t)b;
+  }
+  if (lane == 0) {
+    const long long tok = a.tokens64 ? static_cast<const long long*>(a.tokens)[row] : static_cast<const int*>(a.tokens)[row];
+    float lp = 0.f;
+    if (tok != a.ignore) lp = TNNB_CHECK(tok, a.V) && tok >= 0 && tok < a.V ? log_prob(to_f32(z[tok])) : NAN;
+    a.logp[row] = lp;
+    a.entropy[row] = bad ? NAN : dead ? 0.f : (float)fmax((ls - (double)all.t / all.s) * ln2, 0.0);
+    if (a.stats) {
+      a.stats[2 * row] = bad ? NAN : all.m;
+      a.stats[2 * row + 1] = dead ? 0.f : (float)ls;
+    }
+  }
+}
+
 // `parts` CTAs (a cluster, where more than one) work on a row. Few rows are split so that more of the GPU's loads are in flight.
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS)
+__global__ void __launch_bounds__(LP_THREADS, 4)
 token_logprob_kernel(const LogprobParams a, int parts) {
   constexpr int PER = 16 / sizeof(T), AHEAD = 4;
   __shared__ LogprobShared sh;
@@ -255,23 +345,31 @@ token_logprob_kernel(const LogprobParams a, int parts) {
   r.z = static_cast<const T*>(a.z) + row * a.ld;
   r.p = split_row(r.z, a.V, rank, parts);
 
-  // ---- the pass
-  Sums sum = {-INFINITY, 0.f, 0.f};
-  float mc = 0.f;  // sum.m * c
+  // ---- the pass: sums of even and odd elements side by side in pairs, two pairs of each; the next loads are on their way
+  // while these are worked on
+  float m = -INFINITY, mc = 0.f;  // the largest logit so far, and times c
+  uint64_t s2[2] = {0, 0}, t2[2] = {0, 0};
+  const uint64_t c2 = both_f2(a.c);
   auto raise = [&](float to) {  // a new maximum (or NaN, which stays)
-    to = max_nan(sum.m, to);
-    const float d = rescale(sum.m, to, a.c), f = exp2f(d);
-    sum = {to, sum.s * f, f * (sum.t + sum.s * d)};
+    to = max_nan(m, to);
+    const float d = rescale(m, to, a.c);
+    const uint64_t d2 = both_f2(d), f2 = both_f2(exp2f(d));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      t2[i] = mul_f2(f2, fma_f2(s2[i], d2, t2[i]));
+      s2[i] = mul_f2(s2[i], f2);
+    }
+    m = to;
     mc = __fmul_rn(to, a.c);
   };
-  auto add = [&](float d) {
-    d = fmaxf(d, LP_FLOOR);
-    const float e = exp2f(d);
-    sum.s += e;
-    sum.t = fmaf(e, d, sum.t);
+  auto add = [&](uint64_t d2, int i) {
+    float d0, d1;
+    unpack_f2(d2, d0, d1);
+    const uint64_t e2 = pack_f2(exp2f(d0), exp2f(d1));
+    s2[i] = add_f2(s2[i], e2);
+    t2[i] = fma_f2(e2, d2, t2[i]);
   };
-  for (int v0 = r.p.v_lo + tid; v0 < r.p.v_hi; v0 += LP_THREADS * AHEAD) {
-    Vec<T, PER> v[AHEAD];
+  auto load = [&](Vec<T, PER> (&v)[AHEAD], int v0) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       if (v0 + u * LP_THREADS < r.p.v_hi) {
@@ -281,27 +379,53 @@ token_logprob_kernel(const LogprobParams a, int parts) {
         for (int j = 0; j < PER; ++j) v[u].v[j] = from_f32<T>(-INFINITY);
       }
     }
+  };
+  auto work = [&](const Vec<T, PER> (&v)[AHEAD]) {
     float g = vec_max(v[0]);
 #pragma unroll
     for (int u = 1; u < AHEAD; ++u) g = max_nan(g, vec_max(v[u]));
-    if (!(g <= sum.m)) raise(g);
-    if (!huge(sum.m)) {
+    if (!(g <= m)) raise(g);
+    if (!huge(m)) {
+      const uint64_t nm2 = both_f2(-mc);
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
+      for (int u = 0; u < AHEAD; ++u) {
+        uint64_t x[PER / 2];
+        vec_pairs(v[u], x);
 #pragma unroll
-        for (int j = 0; j < PER; ++j) add(fmaf(to_f32(v[u].v[j]), a.c, -mc));
+        for (int j = 0; j < PER / 2; ++j) add(fma_f2(x[j], c2, nm2), j & 1);
+      }
     } else {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-        for (int j = 0; j < PER; ++j) add((to_f32(v[u].v[j]) - sum.m) * a.c);
+        for (int j = 0; j < PER; j += 2)
+          add(pack_f2(fmaxf((to_f32(v[u].v[j]) - m) * a.c, LP_FLOOR), fmaxf((to_f32(v[u].v[j + 1]) - m) * a.c, LP_FLOOR)), 0);
     }
+  };
+  constexpr int ROUND = LP_THREADS * AHEAD;
+  Vec<T, PER> va[AHEAD], vb[AHEAD];
+  int v0 = r.p.v_lo + tid;
+  load(va, v0);
+  while (v0 < r.p.v_hi) {
+    load(vb, v0 + ROUND);
+    work(va);
+    v0 += ROUND;
+    if (v0 >= r.p.v_hi) break;
+    load(va, v0 + ROUND);
+    work(vb);
+    v0 += ROUND;
+  }
+  Sums sum;
+  {
+    float s0, s1, t0, t1;
+    unpack_f2(add_f2(s2[0], s2[1]), s0, s1);
+    unpack_f2(add_f2(t2[0], t2[1]), t0, t1);
+    sum = {m, s0 + s1, t0 + t1};
   }
   const int single = loose<T>(r.p, tid);
   if (single >= 0) {
-    const float z = r.one(single);
-    if (!(z <= sum.m)) raise(z);
-    add(exponent(z, sum.m, a.c));
+    const float z = r.one(single), d = huge(z) ? 0.f : fmaf(z, a.c, -__fmul_rn(z, a.c)), e = exp2f(d);  // as in the pass: z c - (z c rounded)
+    sum = join(sum, {z, e, e * d}, a.c);
   }
 
   // ---- the bound for the alternatives, and the block's statistics
@@ -338,29 +462,7 @@ token_logprob_kernel(const LogprobParams a, int parts) {
       if (place == k - 1) sh.bound = g;
     }
     __syncthreads();
-    const uint32_t bound = sh.bound;
-    if (own_key >= bound && !nothing) sh.winner[atomicAdd(&sh.winners, 1)] = tid;
-    __syncthreads();
-    const int each = (r.p.v_hi - r.p.v_lo + LP_THREADS - 1) / LP_THREADS + 1;  // a thread's vectors and its loose element
-    for (int it = tid; it < sh.winners * each; it += LP_THREADS) {
-      const int w = sh.winner[it / each], q = it % each;
-      if (q < each - 1) {
-        const int v = r.p.v_lo + w + q * LP_THREADS;
-        if (v >= r.p.v_hi) continue;
-        const Vec<T, PER> x = r.vec(v);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const uint32_t key = key_of(to_f32(x.v[j]));
-          if (key >= bound) add_candidate(sh, key, r.p.head + v * PER + j);
-        }
-      } else {
-        const int i = loose<T>(r.p, w);
-        if (i >= 0 && key_of(r.one(i)) >= bound) add_candidate(sh, key_of(r.one(i)), i);
-      }
-    }
-    __syncthreads();
-    int n = sh.found;
-    if (n > LP_CAND) n = select_by_bisection(r, k, bound, sh);
+    const int n = select_candidates(r, k, own_key, sh);
     rank_candidates(sh.cand, n, k, sh.best);
   }
   __syncthreads();
@@ -388,31 +490,8 @@ token_logprob_kernel(const LogprobParams a, int parts) {
         __syncthreads();
       }
     }
-    const bool dead = all.m == -INFINITY, bad = !(all.m < INFINITY);  // NaN or +inf among the logits
-    const double ls = log2((double)all.s);
-    const double ln2 = 0.69314718055994530942;
-    auto log_prob = [&](float z) -> float {
-      if (bad) return NAN;
-      if (dead || z == -INFINITY) return -INFINITY;
-      const double d = huge(all.m) ? ((double)z - all.m) * a.c : (double)z * a.c - __fmul_rn(all.m, a.c);
-      return (float)((d - ls) * ln2);
-    };
-    if (tid < a.top) {
-      const unsigned long long b = best[tid];
-      a.top_logp[row * a.top + tid] = log_prob(value_of((uint32_t)(b >> 32)));
-      a.top_index[row * a.top + tid] = (long long)(uint32_t)~(uint32_t)b;
-    }
-    if (tid == 0) {
-      const long long tok = a.tokens64 ? static_cast<const long long*>(a.tokens)[row] : static_cast<const int*>(a.tokens)[row];
-      float lp = 0.f;
-      if (tok != a.ignore) lp = TNNB_CHECK(tok, a.V) && tok >= 0 && tok < a.V ? log_prob(to_f32(r.z[tok])) : NAN;
-      a.logp[row] = lp;
-      a.entropy[row] = bad ? NAN : dead ? 0.f : (float)fmax((ls - (double)all.t / all.s) * ln2, 0.0);
-      if (a.stats) {
-        a.stats[2 * row] = bad ? NAN : all.m;
-        a.stats[2 * row + 1] = dead ? 0.f : (float)ls;
-      }
-    }
+    if (warp == 0) write_row(a, all, best, row, r.z);
+    __syncwarp();
   }
   if (parts > 1) cluster_sync_all();  // no CTA leaves while its lists are read
 }
@@ -454,25 +533,27 @@ token_logprob_grad_kernel(const LogprobGradParams a) {
   const float h = a.g_entropy && !dead ? a.g_entropy[row] : 0.f;
   if (tok != a.ignore && !(tok >= 0 && tok < a.V)) g = NAN;  // such a token's log probability is NaN
   const float A = -(g + h * H) * a.inv_temp, B = -h * 0.69314718055994530942f * a.inv_temp, at_token = g * a.inv_temp;
-  // exponent() with the choice made once: (x - sub) c - mc
-  const float sub = huge(m) ? m : 0.f, mc = huge(m) ? 0.f : __fmul_rn(m, a.c);
-  auto grad = [&](float x, int j) {
-    const float d = fmaxf(fmaf(x - sub, a.c, -mc) - ls, LP_FLOOR);
-    float v = exp2f(d) * fmaf(B, d, A);
-    if (j == tok) v += at_token;
-    return dead ? 0.f : v;
-  };
-  if (m != m) {  // NaN statistics make the whole row NaN (fmaxf above would drop it)
-    for (int j = part * 256 + threadIdx.x; j < a.V; j += a.splits * 256) dz[j] = from_f32<T>(NAN);
+  if (m != m || dead) {  // NaN statistics make the whole row NaN
+    const T v = from_f32<T>(dead ? 0.f : NAN);
+    for (int j = part * 256 + threadIdx.x; j < a.V; j += a.splits * 256) dz[j] = v;
     return;
   }
-  if (((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) != 0) {  // rows that cannot share vectors
-    for (int j = part * 256 + threadIdx.x; j < a.V; j += a.splits * 256) dz[j] = from_f32<T>(grad(to_f32(z[j]), j));
+  // log2 p = (x - m) c - (log2 s, less what the rounding of m c took off the sum's exponents)
+  const float off = fmaf(m, a.c, -__fmul_rn(m, a.c)) - ls;
+  const bool big = huge(m);
+  auto one = [&](float x, int j) {
+    const float d = fmaxf(fmaf(x - m, a.c, big ? -ls : off), LP_FLOOR);
+    const float v = exp2f(d) * fmaf(B, d, A);
+    return j == tok ? v + at_token : v;
+  };
+  if (big || ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) != 0) {  // rows that cannot share vectors
+    for (int j = part * 256 + threadIdx.x; j < a.V; j += a.splits * 256) dz[j] = from_f32<T>(one(to_f32(z[j]), j));
     return;
   }
   const RowPart p = split_row(z, a.V, part, a.splits);
   const int single = loose<T>(p, threadIdx.x);
-  if (single >= 0) dz[single] = from_f32<T>(grad(to_f32(z[single]), single));
+  if (single >= 0) dz[single] = from_f32<T>(one(to_f32(z[single]), single));
+  const uint64_t nm2 = both_f2(-m), c2 = both_f2(a.c), off2 = both_f2(off), A2 = both_f2(A), B2 = both_f2(B);
   for (int v0 = p.v_lo + threadIdx.x; v0 < p.v_hi; v0 += 256 * AHEAD) {
     Vec<T, PER> v[AHEAD];
 #pragma unroll
@@ -482,9 +563,21 @@ token_logprob_grad_kernel(const LogprobGradParams a) {
     for (int u = 0; u < AHEAD; ++u) {
       const int vi = v0 + u * 256;
       if (vi >= p.v_hi) break;
+      uint64_t x[PER / 2];
+      vec_pairs(v[u], x);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) v[u].v[j] = from_f32<T>(grad(to_f32(v[u].v[j]), p.head + vi * PER + j));
-      *reinterpret_cast<Vec<T, PER>*>(dz + p.head + vi * PER) = v[u];
+      for (int j = 0; j < PER / 2; ++j) {
+        const uint64_t d2 = fma_f2(add_f2(x[j], nm2), c2, off2);
+        float d0, d1, g0, g1;
+        unpack_f2(d2, d0, d1);
+        unpack_f2(mul_f2(pack_f2(exp2f(d0), exp2f(d1)), fma_f2(B2, d2, A2)), g0, g1);
+        v[u].v[2 * j] = from_f32<T>(g0);
+        v[u].v[2 * j + 1] = from_f32<T>(g1);
+      }
+      T* d = dz + p.head + vi * PER;
+      *reinterpret_cast<Vec<T, PER>*>(d) = v[u];
+      const long long at = tok - p.head - (long long)vi * PER;  // the token's element, by the thread that has just written it
+      if (at >= 0 && at < PER) d[at] = from_f32<T>(one(to_f32(z[tok]), (int)tok));
     }
   }
 }
