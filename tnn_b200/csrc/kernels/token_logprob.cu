@@ -30,6 +30,7 @@ static constexpr int LP_TOP = 32;      // most alternatives
 static constexpr int LP_GROUPS = 64;   // groups of threads whose maxima bound the k-th value
 static constexpr int LP_CAND = 1024;   // candidates that fit
 static constexpr int LP_CLUSTER = 8;   // most CTAs per row
+static constexpr float LP_SLACK = 8.f;
 static constexpr float LP_FLOOR = -1000.f;  // 2^-1000 = 0; finite, so that 0 * exponent is 0 and not NaN
 
 struct LogprobParams {
@@ -45,7 +46,7 @@ struct LogprobParams {
   float* entropy;
   float* top_logp;
   long long* top_index;
-  float* stats;  // [rows][2]: the largest logit, log2 s (null: not wanted)
+  float* stats;  // [rows][2]: what exponents are relative to, log2 s (null: not wanted)
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -53,40 +54,89 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// A vector's largest value, and its elements as pairs of fp32 that -inf has left (0 * -inf would be NaN): at least LP_LOWEST, whose
-// probability beside any logit that huge() lets pass is 0 as well. fp16 cannot hold that bound and is raised to it afterwards.
+// 16 bytes of logits as four words: the largest value (NaN if there is one), and the elements as pairs of fp32 that -inf has left
+// (0 * -inf would be NaN): at least LP_LOWEST, whose probability beside any logit that huge() lets pass is 0 as well. (fp16 cannot hold
+// that bound and is raised to it afterwards.) Whole words throughout: as arrays of 16-bit elements the same took twice the instructions.
 static constexpr float LP_LOWEST = -1e20f;
-__device__ __forceinline__ float vec_max(const Vec<float, 4>& v) { return max_nan(max_nan(v.v[0], v.v[1]), max_nan(v.v[2], v.v[3])); }
-__device__ __forceinline__ void vec_pairs(const Vec<float, 4>& v, uint64_t (&x)[2]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) x[i] = pack_f2(fmaxf(v.v[2 * i], LP_LOWEST), fmaxf(v.v[2 * i + 1], LP_LOWEST));
-}
-__device__ __forceinline__ float vec_max(const Vec<__nv_bfloat16, 8>& v) {
-  const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(v.v);
-  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
-  return max_nan(__low2float(m), __high2float(m));
-}
-__device__ __forceinline__ void vec_pairs(const Vec<__nv_bfloat16, 8>& v, uint64_t (&x)[4]) {
-  const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(v.v);
-  const __nv_bfloat162 lowest = __float2bfloat162_rn(LP_LOWEST);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 m = __hmax2(w[i], lowest);
-    x[i] = bf16x2_to_f2(*reinterpret_cast<const uint32_t*>(&m));
+template <typename T> struct Logits;
+template <>
+struct Logits<float> {
+  static constexpr uint32_t NONE = 0xff800000u;  // -inf
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
+  static __device__ __forceinline__ float largest(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[2]) {
+    x[0] = pack_f2(fmaxf(__uint_as_float(v.x), LP_LOWEST), fmaxf(__uint_as_float(v.y), LP_LOWEST));
+    x[1] = pack_f2(fmaxf(__uint_as_float(v.z), LP_LOWEST), fmaxf(__uint_as_float(v.w), LP_LOWEST));
   }
-}
-__device__ __forceinline__ float vec_max(const Vec<__half, 8>& v) {
-  const __half2* w = reinterpret_cast<const __half2*>(v.v);
-  const __half2 m = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
-  return max_nan(__low2float(m), __high2float(m));
-}
-__device__ __forceinline__ void vec_pairs(const Vec<__half, 8>& v, uint64_t (&x)[4]) {
-  const __half2* w = reinterpret_cast<const __half2*>(v.v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(w[i]);
-    x[i] = pack_f2(fmaxf(f.x, LP_LOWEST), fmaxf(f.y, LP_LOWEST));
+  static __device__ __forceinline__ void values(uint32_t w, float (&x)[1]) { x[0] = __uint_as_float(w); }
+  static __device__ __forceinline__ void put(uint4& v, int pair, float a, float b) {
+    reinterpret_cast<uint32_t*>(&v)[2 * pair] = __float_as_uint(a), reinterpret_cast<uint32_t*>(&v)[2 * pair + 1] = __float_as_uint(b);
   }
+};
+template <>
+struct Logits<__nv_bfloat16> {
+  static constexpr uint32_t NONE = 0xff80ff80u;
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float largest(uint32_t w) { return max_nan(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+  static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[4]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t r;
+      asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w[i]), "r"(0xe0aee0aeu));  // the bf16 next below LP_LOWEST, twice
+      x[i] = bf16x2_to_f2(r);
+    }
+  }
+  static __device__ __forceinline__ void values(uint32_t w, float (&x)[2]) {
+    x[0] = __uint_as_float(w << 16), x[1] = __uint_as_float(w & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void put(uint4& v, int pair, float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    reinterpret_cast<uint32_t*>(&v)[pair] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Logits<__half> {
+  static constexpr uint32_t NONE = 0xfc00fc00u;
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ void values(uint32_t w, float (&x)[2]) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    x[0] = f.x, x[1] = f.y;
+  }
+  static __device__ __forceinline__ float largest(uint32_t w) {
+    float x[2];
+    values(w, x);
+    return max_nan(x[0], x[1]);
+  }
+  static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[4]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[2];
+      values(w[i], f);
+      x[i] = pack_f2(fmaxf(f[0], LP_LOWEST), fmaxf(f[1], LP_LOWEST));
+    }
+  }
+  static __device__ __forceinline__ void put(uint4& v, int pair, float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    reinterpret_cast<uint32_t*>(&v)[pair] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <typename T, int N>
+__device__ __forceinline__ float vec_max(const uint4 (&v)[N]) {
+  using L = Logits<T>;
+  uint32_t m = L::larger(L::larger(v[0].x, v[0].y), L::larger(v[0].z, v[0].w));
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = L::larger(m, L::larger(L::larger(v[i].x, v[i].y), L::larger(v[i].z, v[i].w)));
+  return L::largest(m);
 }
 
 // Order of logits as unsigned integers (0: none at all), NaN above +inf, -0 equal to +0.
@@ -108,7 +158,8 @@ __device__ __forceinline__ float rescale(float m, float to, float c) {
   return fmaxf(d, LP_FLOOR);
 }
 
-// Maximum logit of a set of elements, the sum of 2^d and the sum of 2^d d for their exponents d.
+// Of a set of elements: the sum of 2^d and the sum of 2^d d for their exponents d relative to m, the largest logit or one not far
+// below it (-inf: there are only such; NaN, +inf: the set holds one).
 struct Sums {
   float m, s, t;
 };
@@ -117,6 +168,22 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c) {
   const float da = rescale(a.m, m, c), db = rescale(b.m, m, c);
   const float fa = exp2f(da), fb = exp2f(db);
   return {m, a.s * fa + b.s * fb, fa * (a.t + a.s * da) + fb * (b.t + b.s * db)};
+}
+
+// The sums of N neighbouring lanes; every lane gets the same bits.
+template <int N>
+__device__ __forceinline__ Sums join_lanes(const Sums& a, float c) {
+  float m = a.m;
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float d = rescale(a.m, m, c), f = exp2f(d);
+  float s = a.s * f, t = f * (a.t + a.s * d);
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    t += __shfl_xor_sync(0xffffffffu, t, o);
+  }
+  return {m, s, t};
 }
 
 __device__ __forceinline__ float cluster_load(const void* own, int rank) {
@@ -130,7 +197,24 @@ __device__ __forceinline__ unsigned long long cluster_load64(const void* own, in
   return v;
 }
 
+// The pass keeps LP_RING - 1 groups of LP_VECS vectors per thread on their way through shared memory (cp.async; every thread
+// reads its own only). Through registers, with no more in flight than those hold beside the sums, rows came in at 5.2 TB/s
+// even where nothing was computed from them.
+static constexpr int LP_VECS = 2, LP_RING = 4;
+__device__ __forceinline__ void copy16_async(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 struct LogprobShared {
+  union {
+    uint4 ring[LP_RING][LP_VECS][LP_THREADS];  // until the row has been read
+    unsigned long long cand[LP_CAND];
+  };
   uint32_t group[LP_GROUPS];
   uint32_t bound;
   int winners, found, total;
@@ -139,7 +223,6 @@ struct LogprobShared {
   Sums part[LP_THREADS / 32];
   Sums all;
   unsigned long long best[LP_TOP];  // this CTA's, in order; 0 past the last
-  unsigned long long cand[LP_CAND];
 };
 
 // A row's part: elements [head_lo, head_hi) and [tail_lo, tail_hi) one by one, vectors [v_lo, v_hi) between (vector v begins at
@@ -332,9 +415,9 @@ __device__ __forceinline__ void write_row(const LogprobParams& a, const Sums& al
 
 // `parts` CTAs (a cluster, where more than one) work on a row. Few rows are split so that more of the GPU's loads are in flight.
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 4)
+__global__ void __launch_bounds__(LP_THREADS, 5)
 token_logprob_kernel(const LogprobParams a, int parts) {
-  constexpr int PER = 16 / sizeof(T), AHEAD = 4;
+  constexpr int PER = 16 / sizeof(T);
   __shared__ LogprobShared sh;
   grid_dep_launch();
   grid_dep_wait();
@@ -346,11 +429,13 @@ token_logprob_kernel(const LogprobParams a, int parts) {
   r.p = split_row(r.z, a.V, rank, parts);
 
   // ---- the pass: sums of even and odd elements side by side in pairs, two pairs of each; the next loads are on their way
-  // while these are worked on
-  float m = -INFINITY, mc = 0.f;  // the largest logit so far, and times c
+  // while these are worked on. Exponents are relative to the warp's largest logit of its first round; only one that lies LP_SLACK
+  // above (in base 2) moves that, or nearly every round some lane would, and the warp with it.
+  float top = -INFINITY;           // this thread's largest logit
+  float m = -INFINITY, mc = 0.f;  // what exponents are relative to, and times c
   uint64_t s2[2] = {0, 0}, t2[2] = {0, 0};
   const uint64_t c2 = both_f2(a.c);
-  auto raise = [&](float to) {  // a new maximum (or NaN, which stays)
+  auto raise = [&](float to) {  // (NaN stays)
     to = max_nan(m, to);
     const float d = rescale(m, to, a.c);
     const uint64_t d2 = both_f2(d), f2 = both_f2(exp2f(d));
@@ -369,51 +454,69 @@ token_logprob_kernel(const LogprobParams a, int parts) {
     s2[i] = add_f2(s2[i], e2);
     t2[i] = fma_f2(e2, d2, t2[i]);
   };
-  auto load = [&](Vec<T, PER> (&v)[AHEAD], int v0) {
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      if (v0 + u * LP_THREADS < r.p.v_hi) {
-        v[u] = r.vec(v0 + u * LP_THREADS);
-      } else {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) v[u].v[j] = from_f32<T>(-INFINITY);
-      }
-    }
-  };
-  auto work = [&](const Vec<T, PER> (&v)[AHEAD]) {
-    float g = vec_max(v[0]);
-#pragma unroll
-    for (int u = 1; u < AHEAD; ++u) g = max_nan(g, vec_max(v[u]));
-    if (!(g <= m)) raise(g);
+  auto work = [&](const uint4 (&v)[LP_VECS]) {
+    const float g = vec_max<T>(v);
+    top = max_nan(top, g);
+    if (huge(m) ? !(g <= m) : !(fmaf(g, a.c, -mc) <= LP_SLACK)) raise(g);
     if (!huge(m)) {
       const uint64_t nm2 = both_f2(-mc);
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
+      for (int u = 0; u < LP_VECS; ++u) {
         uint64_t x[PER / 2];
-        vec_pairs(v[u], x);
+        Logits<T>::pairs(v[u], x);
 #pragma unroll
         for (int j = 0; j < PER / 2; ++j) add(fma_f2(x[j], c2, nm2), j & 1);
       }
     } else {
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
+      for (int u = 0; u < LP_VECS; ++u) {
+        const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
-        for (int j = 0; j < PER; j += 2)
-          add(pack_f2(fmaxf((to_f32(v[u].v[j]) - m) * a.c, LP_FLOOR), fmaxf((to_f32(v[u].v[j + 1]) - m) * a.c, LP_FLOOR)), 0);
+        for (int j = 0; j < 4; ++j) {
+          float x[PER / 4];
+          Logits<T>::values(w[j], x);
+#pragma unroll
+          for (int i = 0; i < PER / 4; ++i) add(pack_f2(fmaxf((x[i] - m) * a.c, LP_FLOOR), LP_FLOOR), 0);
+        }
+      }
     }
   };
-  constexpr int ROUND = LP_THREADS * AHEAD;
-  Vec<T, PER> va[AHEAD], vb[AHEAD];
-  int v0 = r.p.v_lo + tid;
-  load(va, v0);
-  while (v0 < r.p.v_hi) {
-    load(vb, v0 + ROUND);
-    work(va);
-    v0 += ROUND;
-    if (v0 >= r.p.v_hi) break;
-    load(va, v0 + ROUND);
-    work(vb);
-    v0 += ROUND;
+  constexpr int ROUND = LP_THREADS * LP_VECS, DEPTH = LP_RING - 1;
+  const int vecs = r.p.v_hi - r.p.v_lo;
+  const T* from = r.z + r.p.head + (r.p.v_lo + tid) * PER;  // this thread's vectors of the next round to request
+  int left = vecs - tid;                                    // > 0, > LP_THREADS, ...: as many of them exist
+  auto request = [&](int slot) {
+#pragma unroll
+    for (int u = 0; u < LP_VECS; ++u)
+      if (u * LP_THREADS < left) copy16_async(&sh.ring[slot][u][tid], from + u * (LP_THREADS * PER));
+    copy_commit();
+    from += ROUND * PER;
+    left -= ROUND;
+  };
+  auto take = [&](int slot, uint4 (&v)[LP_VECS]) {
+    copy_wait<DEPTH - 1>();
+#pragma unroll
+    for (int u = 0; u < LP_VECS; ++u) v[u] = sh.ring[slot][u][tid];
+  };
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) request(i);
+  const int rounds = (vecs + ROUND - 1) / ROUND;
+  for (int i = 0; i < rounds; ++i) {
+    uint4 v[LP_VECS];
+    take(i % LP_RING, v);
+    if (i + 1 == rounds) {  // vectors that do not exist
+#pragma unroll
+      for (int u = 0; u < LP_VECS; ++u)
+        if (i * ROUND + u * LP_THREADS + tid >= vecs) v[u] = make_uint4(Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE);
+    }
+    request((i + DEPTH) % LP_RING);
+    if (i == 0) {
+      float first = vec_max<T>(v);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) first = max_nan(first, __shfl_xor_sync(0xffffffffu, first, o));
+      raise(first);
+    }
+    work(v);
   }
   Sums sum;
   {
@@ -426,12 +529,13 @@ token_logprob_kernel(const LogprobParams a, int parts) {
   if (single >= 0) {
     const float z = r.one(single), d = huge(z) ? 0.f : fmaf(z, a.c, -__fmul_rn(z, a.c)), e = exp2f(d);  // as in the pass: z c - (z c rounded)
     sum = join(sum, {z, e, e * d}, a.c);
+    top = max_nan(top, z);
   }
 
   // ---- the bound for the alternatives, and the block's statistics
   const int k = min(a.top, r.p.hi - r.p.lo);
   const bool nothing = tid >= r.p.v_hi - r.p.v_lo && single < 0;
-  const uint32_t own_key = nothing ? 0u : key_of(sum.m);
+  const uint32_t own_key = nothing ? 0u : key_of(top);
   if (k > 0) {
     uint32_t g = own_key;
 #pragma unroll
@@ -440,19 +544,12 @@ token_logprob_kernel(const LogprobParams a, int parts) {
     if (tid < LP_TOP) sh.best[tid] = 0;
     if (tid == 0) sh.winners = sh.found = 0;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums other = {__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o),
-                        __shfl_xor_sync(0xffffffffu, sum.t, o)};
-    // the lower lane's sums first in both lanes of a pair, so that both get the same bits
-    sum = (lane & o) ? join(other, sum, a.c) : join(sum, other, a.c);
-  }
+  sum = join_lanes<32>(sum, a.c);
   if (lane == 0) sh.part[warp] = sum;
   __syncthreads();
-  if (warp == LP_THREADS / 32 - 1 && lane == 0) {
-    Sums all = sh.part[0];
-    for (int w = 1; w < LP_THREADS / 32; ++w) all = join(all, sh.part[w], a.c);
-    sh.all = all;
+  if (warp == 0) {
+    sum = join_lanes<LP_THREADS / 32>(sh.part[lane % (LP_THREADS / 32)], a.c);
+    if (parts > 1 && lane == 0) sh.all = sum;
   }
   if (k > 0) {
     if (tid < LP_GROUPS) {
@@ -464,16 +561,16 @@ token_logprob_kernel(const LogprobParams a, int parts) {
     __syncthreads();
     const int n = select_candidates(r, k, own_key, sh);
     rank_candidates(sh.cand, n, k, sh.best);
+    __syncthreads();
   }
-  __syncthreads();
 
   // ---- the row's results, by the first CTA
   if (parts > 1) cluster_sync_all();
   if (rank == 0) {
-    Sums all = sh.all;
+    Sums all = sum;  // (warp 0's)
     const unsigned long long* best = sh.best;
     if (parts > 1) {
-      for (int q = 1; q < parts; ++q) {
+      for (int q = 1; warp == 0 && q < parts; ++q) {
         const Sums* there = &sh.all;
         const Sums other = {cluster_load(&there->m, q), cluster_load(&there->s, q), cluster_load(&there->t, q)};
         all = join(all, other, a.c);
@@ -555,27 +652,26 @@ token_logprob_grad_kernel(const LogprobGradParams a) {
   if (single >= 0) dz[single] = from_f32<T>(one(to_f32(z[single]), single));
   const uint64_t nm2 = both_f2(-m), c2 = both_f2(a.c), off2 = both_f2(off), A2 = both_f2(A), B2 = both_f2(B);
   for (int v0 = p.v_lo + threadIdx.x; v0 < p.v_hi; v0 += 256 * AHEAD) {
-    Vec<T, PER> v[AHEAD];
+    uint4 v[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-      if (v0 + u * 256 < p.v_hi) v[u] = *reinterpret_cast<const Vec<T, PER>*>(z + p.head + (v0 + u * 256) * PER);
+      if (v0 + u * 256 < p.v_hi) v[u] = *reinterpret_cast<const uint4*>(z + p.head + (v0 + u * 256) * PER);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int vi = v0 + u * 256;
       if (vi >= p.v_hi) break;
       uint64_t x[PER / 2];
-      vec_pairs(v[u], x);
+      Logits<T>::pairs(v[u], x);
 #pragma unroll
       for (int j = 0; j < PER / 2; ++j) {
         const uint64_t d2 = fma_f2(add_f2(x[j], nm2), c2, off2);
         float d0, d1, g0, g1;
         unpack_f2(d2, d0, d1);
         unpack_f2(mul_f2(pack_f2(exp2f(d0), exp2f(d1)), fma_f2(B2, d2, A2)), g0, g1);
-        v[u].v[2 * j] = from_f32<T>(g0);
-        v[u].v[2 * j + 1] = from_f32<T>(g1);
+        Logits<T>::put(v[u], j, g0, g1);
       }
       T* d = dz + p.head + vi * PER;
-      *reinterpret_cast<Vec<T, PER>*>(d) = v[u];
+      *reinterpret_cast<uint4*>(d) = v[u];
       const long long at = tok - p.head - (long long)vi * PER;  // the token's element, by the thread that has just written it
       if (at >= 0 && at < PER) d[at] = from_f32<T>(one(to_f32(z[tok]), (int)tok));
     }
