@@ -53,55 +53,70 @@ embed_lookup_kernel(const ID* __restrict__ ids, const T* __restrict__ table, lon
 }
 
 // -------------------------------------------------------------------------------------------------------------- sort
-// Positions sorted by token, stable, without a pass over global counters: every CTA owns a range of table rows, reads ALL ids
-// (they come from L2: 64 KB for 8192 tokens) and picks its own. The number of ids below its range is the place of its part of the
-// list, so no CTA waits for another. Within the CTA each warp walks a contiguous stretch of the ids and has a counter per row:
-// counts, then starting places (rows ascending, warps ascending within a row), then the places themselves. Rows nobody names are
-// cleared here, by the CTA that knows, so that the whole table's gradient is written exactly once.
+// Positions sorted by token, stable, without a pass over global counters: every CTA owns some table rows, reads ALL ids (they come
+// from L2: 64 KB for 8192 tokens) and picks its own. The number of ids that belong to CTAs before it is the place of its part of
+// the list, so no CTA waits for another. Within the CTA each warp walks a contiguous stretch of the ids and has a counter per row:
+// counts, then starting places (rows ascending, warps ascending within a row), then the places themselves. A place gets its token with
+// two flags, so that what adds up needs no other table: whether it is the token's first position and whether it is its last.
+//
+// Rows are dealt out in turn (2^bits CTAs; row v is number v >> bits of CTA v mod 2^bits): frequent tokens have neighbouring numbers, and
+// with ranges of rows the CTA that had them took 16 us for 8192 tokens of text, 63 for 50001. The list is in this order of rows
+// ("slots"), which is as good as any.
 static constexpr int SORT_WARPS = 32;
 static constexpr int SORT_ROWS = 512;  // most rows of a CTA: 64 KB of counters, two CTAs per SM
+static constexpr uint32_t TOKEN_FIRST = 1u << 30, TOKEN_LAST = 1u << 31, TOKEN_ROW = TOKEN_FIRST - 1;
+
+struct Slots {
+  int bits, rows;  // rows per CTA, those past the table included
+};
+__host__ __device__ __forceinline__ Slots slots_of(long long vocab) {
+  Slots s;
+  s.bits = 0;
+  while (s.bits < 7 && (1ll << s.bits) < vocab) ++s.bits;                          // 128 CTAs
+  while (((vocab + (1ll << s.bits) - 1) >> s.bits) > SORT_ROWS) ++s.bits;
+  s.rows = (int)((vocab + (1ll << s.bits) - 1) >> s.bits);
+  return s;
+}
+__device__ __forceinline__ int slot_of(const Slots& s, int row) { return (row & ((1 << s.bits) - 1)) * s.rows + (row >> s.bits); }
 
 template <typename ID>
-__device__ __forceinline__ long long sort_row(const ID* ids, int i, long long vocab, long long padding) {
+__device__ __forceinline__ int sort_row(const ID* ids, int i, long long vocab, long long padding) {
   const long long id = ids[i];
   if (id == padding) return -1;
   (void)TNNB_CHECK(id, vocab);
-  return id < 0 || id >= vocab ? 0 : id;
+  return id < 0 || id >= vocab ? 0 : (int)id;
 }
 
 template <typename ID>
 __global__ void __launch_bounds__(SORT_WARPS * 32)
-embed_sort_kernel(const ID* ids, int n, long long vocab, long long padding, int rows_each,
-                                                                     int* order, int* keys, int* rowptr, uint8_t* clear,
-                                                                     long long row_bytes) {
+embed_sort_kernel(const ID* ids, int n, long long vocab, long long padding, Slots slots, int* order, uint32_t* keys, int* rowptr) {
   grid_dep_launch();
   grid_dep_wait();
-  extern __shared__ int counters[];  // [SORT_WARPS][rows_each]
+  extern __shared__ int counters[];  // [SORT_WARPS][slots.rows]
   __shared__ int below[SORT_WARPS], scan[SORT_WARPS];
-  __shared__ uint8_t empty[SORT_ROWS];
+  __shared__ int begin[SORT_ROWS], count[SORT_ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long v0 = (long long)blockIdx.x * rows_each;
-  const int rows = (int)min((long long)rows_each, vocab - v0);
-  for (int i = threadIdx.x; i < SORT_WARPS * rows_each; i += blockDim.x) counters[i] = 0;
+  const int rows = slots.rows, own = blockIdx.x, mask = (1 << slots.bits) - 1;
+  for (int i = threadIdx.x; i < SORT_WARPS * rows; i += blockDim.x) counters[i] = 0;
   __syncthreads();
 
   const int stretch = ((n + SORT_WARPS - 1) / SORT_WARPS + 31) / 32 * 32;
   const int lo = min((long long)n, (long long)warp * stretch), hi = min((long long)n, (long long)lo + stretch);
-  int* mine = counters + warp * rows_each;
+  int* mine = counters + warp * rows;
   int less = 0;
-  constexpr int AHEAD = 4;
+  constexpr int AHEAD = 8;
   for (int i0 = lo; i0 < hi; i0 += 32 * AHEAD) {
-    long long r[AHEAD];
+    int r[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) r[u] = i0 + u * 32 + lane < hi ? sort_row(ids, i0 + u * 32 + lane, vocab, padding) : -1;
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      less += r[u] >= 0 && r[u] < v0;
-      const bool in = r[u] >= v0 && r[u] < v0 + rows;
+      less += r[u] >= 0 && (r[u] & mask) < own;
+      const bool in = r[u] >= 0 && (r[u] & mask) == own;
       const unsigned who = __ballot_sync(0xffffffffu, in);
       if (who == 0) continue;
       if (in) {
-        const int at = (int)(r[u] - v0);
+        const int at = r[u] >> slots.bits;
         const unsigned same = __match_any_sync(who, at);
         if ((same & ((1u << lane) - 1)) == 0) mine[at] += __popc(same);
       }
@@ -116,8 +131,8 @@ embed_sort_kernel(const ID* ids, int n, long long vocab, long long padding, int 
   int total = 0;
   if ((int)threadIdx.x < rows)
     for (int w = 0; w < SORT_WARPS; ++w) {
-      const int c = counters[w * rows_each + threadIdx.x];
-      counters[w * rows_each + threadIdx.x] = total;
+      const int c = counters[w * rows + threadIdx.x];
+      counters[w * rows + threadIdx.x] = total;
       total += c;
     }
   int upto = total;  // sum over the rows up to this thread's
@@ -131,45 +146,34 @@ embed_sort_kernel(const ID* ids, int n, long long vocab, long long padding, int 
   int start = upto - total;
   for (int w = 0; w < SORT_WARPS; ++w) start += below[w] + (w < warp ? scan[w] : 0);
   if ((int)threadIdx.x < rows) {
-    rowptr[v0 + threadIdx.x] = start;
-    if (v0 + threadIdx.x == vocab - 1) rowptr[vocab] = start + total;
-    for (int w = 0; w < SORT_WARPS; ++w) counters[w * rows_each + threadIdx.x] += start;
-    empty[threadIdx.x] = total == 0;
+    rowptr[own * rows + threadIdx.x] = start;
+    if (own == mask && (int)threadIdx.x == rows - 1) rowptr[(mask + 1) * rows] = start + total;
+    for (int w = 0; w < SORT_WARPS; ++w) counters[w * rows + threadIdx.x] += start;
+    begin[threadIdx.x] = start, count[threadIdx.x] = total;
   }
   __syncthreads();
 
   for (int i0 = lo; i0 < hi; i0 += 32 * AHEAD) {
-    long long r[AHEAD];
+    int r[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) r[u] = i0 + u * 32 + lane < hi ? sort_row(ids, i0 + u * 32 + lane, vocab, padding) : -1;
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const bool in = r[u] >= v0 && r[u] < v0 + rows;
+      const bool in = r[u] >= 0 && (r[u] & mask) == own;
       const unsigned who = __ballot_sync(0xffffffffu, in);
       if (who == 0) continue;
       int at = 0;
       unsigned same = 0;
       if (in) {
-        at = (int)(r[u] - v0);
+        at = r[u] >> slots.bits;
         same = __match_any_sync(who, at);
         const int to = mine[at] + __popc(same & ((1u << lane) - 1));
         order[to] = i0 + u * 32 + lane;
-        keys[to] = (int)r[u];
+        keys[to] = (uint32_t)r[u] | (to == begin[at] ? TOKEN_FIRST : 0u) | (to + 1 == begin[at] + count[at] ? TOKEN_LAST : 0u);
       }
       __syncwarp();
       if (in && (same & ((1u << lane) - 1)) == 0) mine[at] += __popc(same);
       __syncwarp();
-    }
-  }
-  if (clear == nullptr) return;
-  const bool wide = ((reinterpret_cast<uintptr_t>(clear) | row_bytes) & 15) == 0;
-  for (int r = warp; r < rows; r += SORT_WARPS) {
-    if (!empty[r]) continue;
-    uint8_t* row = clear + (v0 + r) * row_bytes;
-    if (wide) {
-      for (long long b = lane * 16; b < row_bytes; b += 32 * 16) *reinterpret_cast<uint4*>(row + b) = make_uint4(0, 0, 0, 0);
-    } else {
-      for (long long b = lane * 2; b < row_bytes; b += 32 * 2) *reinterpret_cast<uint16_t*>(row + b) = 0;  // elements have two bytes or four
     }
   }
 }
@@ -177,65 +181,101 @@ embed_sort_kernel(const ID* ids, int n, long long vocab, long long padding, int 
 // -------------------------------------------------------------------------------------------------------------- sums
 // A CTA takes `chunk` consecutive places of the sorted list, whatever tokens they belong to, so that a frequent token's positions are
 // spread over many CTAs. A token that lies within the chunk is finished; the sum of one that reaches in from the chunk before (part
-// 0) or on into the next (part 1) goes to the workspace, and embed_join_kernel adds those up.
-template <typename TI, typename TO, int VEC>
+// 0) or on into the next (part 1) goes to the workspace, and embed_join_kernel adds those up. The first `fills` CTAs clear the rows
+// that nobody names instead: most of the bytes, written while the others wait for the rows they gather.
+//
+// A thread has COLS vectors of VEC columns, blockDim.x vectors apart (single columns where rows are not aligned: four of them share
+// the bookkeeping).
+__device__ __forceinline__ void clear_row(uint8_t* row, long long bytes, int lane) {  // one warp; addresses are even
+  const int head = (int)min(bytes, (long long)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15));
+  const long long body = (bytes - head) / 16;
+  if (lane * 2 < head) *reinterpret_cast<uint16_t*>(row + lane * 2) = 0;
+  for (long long i = lane; i < body; i += 32) reinterpret_cast<uint4*>(row + head)[i] = make_uint4(0, 0, 0, 0);
+  const long long tail = head + body * 16 + lane * 2;
+  if (tail < bytes) *reinterpret_cast<uint16_t*>(row + tail) = 0;
+}
+
+template <typename TI, typename TO, int VEC, int COLS>
 __global__ void __launch_bounds__(256)
-embed_sum_kernel(const TI* dy, long long ld, const int* order, const int* keys, const int* rowptr,
-                                                        long long vocab, TO* out, float* parts, int width, int chunk, float scale,
-                                                        int accumulate) {
-  extern __shared__ int places[];  // [chunk] positions, [chunk + 1] tokens
+embed_sum_kernel(const TI* dy, long long ld, const int* order, const uint32_t* keys, const int* rowptr, long long vocab, Slots slots,
+                 TO* out, float* parts, int width, int chunk, int fills, float scale, int accumulate) {
+  extern __shared__ int places[];  // [chunk] positions, [chunk] tokens
   grid_dep_launch();
   grid_dep_wait();
-  const int n = rowptr[vocab];
-  const long long first = (long long)blockIdx.x * chunk;
-  if (first >= n) return;
+  if ((int)blockIdx.x < fills) {
+    if (accumulate) return;
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const long long all = (long long)fills * gridDim.y * warps;
+    const long long me = ((long long)blockIdx.y * fills + blockIdx.x) * warps + (threadIdx.x >> 5);
+    for (long long r0 = me * 32; r0 < vocab; r0 += all * 32) {
+      const long long r = r0 + lane;
+      const int at = r < vocab ? slot_of(slots, (int)r) : 0;
+      unsigned empty = __ballot_sync(0xffffffffu, r < vocab && rowptr[at] == rowptr[at + 1]);
+      for (; empty; empty &= empty - 1)
+        clear_row(reinterpret_cast<uint8_t*>(out + (r0 + __ffs(empty) - 1) * width), (long long)width * sizeof(TO), lane);
+    }
+    return;
+  }
+  const int n = rowptr[slots.rows << slots.bits], me = blockIdx.x - fills;
+  const long long first = (long long)me * chunk;
   const int count = (int)min((long long)chunk, n - first);
-  int* token = places + chunk;
+  uint32_t* token = reinterpret_cast<uint32_t*>(places + chunk);
   for (int i = threadIdx.x; i < count; i += blockDim.x) {
     places[i] = order[first + i];
     token[i] = keys[first + i];
   }
-  if (threadIdx.x == 0) token[count] = -1;
   __syncthreads();
-  const int col = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-  if (col >= width) return;
-  const bool from_before = rowptr[token[0]] < first;
-  const bool goes_on = rowptr[token[count - 1] + 1] > first + count;
+  if (count <= 0) return;
+  const int col0 = (blockIdx.y * COLS * blockDim.x + threadIdx.x) * VEC, step = blockDim.x * VEC;
 
   using V = Vec<TI, VEC>;
-  constexpr int AHEAD = 8;
-  float sum[VEC];
+  constexpr int AHEAD = COLS > 1 ? 4 : 8;
+  float sum[COLS][VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-  bool opening = true;  // the chunk's first token
+  for (int c = 0; c < COLS; ++c)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum[c][j] = 0.f;
+  bool from_before = !(token[0] & TOKEN_FIRST);
   for (int i0 = 0; i0 < count; i0 += AHEAD) {
-    V v[AHEAD];
+    V v[AHEAD][COLS];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-      if (i0 + u < count) v[u] = *reinterpret_cast<const V*>(dy + places[i0 + u] * ld + col);
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+        if (i0 + u < count && col0 + c * step < width) v[u][c] = *reinterpret_cast<const V*>(dy + places[i0 + u] * ld + col0 + c * step);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int i = i0 + u;
       if (i >= count) break;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[j] += to_f32(v[u].v[j]);
-      if (token[i + 1] == token[i]) continue;
-      const bool head = opening && from_before, open = head || (i + 1 == count && goes_on);
-      opening = false;
-      if (open) {
-        float* p = parts + (2 * (long long)blockIdx.x + (head ? 0 : 1)) * width + col;
+      for (int c = 0; c < COLS; ++c)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) p[j] = sum[j];
+        for (int j = 0; j < VEC; ++j) sum[c][j] += to_f32(v[u][c].v[j]);
+      const uint32_t t = token[i];
+      if (!(t & TOKEN_LAST) && i + 1 < count) continue;
+      if (from_before || !(t & TOKEN_LAST)) {
+        float* p = parts + (2 * (long long)me + (from_before ? 0 : 1)) * width;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+          if (col0 + c * step < width) *reinterpret_cast<Vec<float, VEC>*>(p + col0 + c * step) = *reinterpret_cast<Vec<float, VEC>*>(sum[c]);
       } else {
-        TO* o = out + (long long)token[i] * width + col;
-        Vec<TO, VEC> r;
-        if (accumulate) r = *reinterpret_cast<const Vec<TO, VEC>*>(o);
+        TO* o = out + (long long)(t & TOKEN_ROW) * width;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) r.v[j] = from_f32<TO>(accumulate ? to_f32(r.v[j]) + sum[j] * scale : sum[j] * scale);
-        *reinterpret_cast<Vec<TO, VEC>*>(o) = r;
+        for (int c = 0; c < COLS; ++c) {
+          if (col0 + c * step >= width) continue;
+          Vec<TO, VEC>* at = reinterpret_cast<Vec<TO, VEC>*>(o + col0 + c * step);
+          Vec<TO, VEC> r;
+          if (accumulate) r = *at;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) r.v[j] = from_f32<TO>(accumulate ? to_f32(r.v[j]) + sum[c][j] * scale : sum[c][j] * scale);
+          *at = r;
+        }
       }
+      from_before = false;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+      for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sum[c][j] = 0.f;
     }
   }
 }
@@ -245,19 +285,21 @@ embed_sum_kernel(const TI* dy, long long ld, const int* order, const int* keys, 
 static constexpr int JOIN_COLS = 128, JOIN_WARPS = 8;
 template <typename TO>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
-embed_join_kernel(const float* parts, const int* keys, const int* rowptr, long long vocab,
-                                                                     TO* out, int width, int chunk, float scale, int accumulate) {
+embed_join_kernel(const float* parts, const uint32_t* keys, const int* rowptr, Slots slots, TO* out, int width, int chunk, float scale,
+                  int accumulate) {
   __shared__ float sums[JOIN_WARPS][JOIN_COLS];
   grid_dep_launch();
   grid_dep_wait();
-  const int n = rowptr[vocab];
+  const int n = rowptr[slots.rows << slots.bits];
   const long long next = ((long long)blockIdx.x + 1) * chunk;
-  if (next >= n) return;
-  const int token = keys[next];
-  if (keys[next - 1] != token || rowptr[token] < next - chunk) return;
-  const int more = (int)((rowptr[token + 1] - 1) / chunk - blockIdx.x);  // chunks after this one
+  if (next >= n || (keys[next - 1] & TOKEN_LAST)) return;
+  const uint32_t token = keys[next - 1] & TOKEN_ROW;
+  const int at = slot_of(slots, (int)token);
+  if (rowptr[at] < next - chunk) return;  // begins in an earlier chunk
+  const int more = (int)((rowptr[at + 1] - 1) / chunk - blockIdx.x);  // chunks after this one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y * JOIN_COLS + lane;
   float s[JOIN_COLS / 32] = {};
+#pragma unroll 8
   for (int k = warp; k <= more; k += JOIN_WARPS) {
     const float* p = parts + (2 * ((long long)blockIdx.x + k) + (k == 0 ? 1 : 0)) * width + col;
 #pragma unroll
@@ -275,45 +317,43 @@ embed_join_kernel(const float* parts, const int* keys, const int* rowptr, long l
   TO* o = out + (long long)token * width + c;
   *o = from_f32<TO>(accumulate ? to_f32(*o) + total * scale : total * scale);
 }
-
 template <typename TI, typename TO>
-static cudaError_t sum_and_join(const void* dy, long long ld, const int* order, const int* keys, const int* rowptr, int n, long long vocab,
-                                void* out, float* parts, int width, int chunk, float scale, int accumulate, cudaStream_t st) {
+static cudaError_t sum_and_join(const void* dy, long long ld, const int* order, const uint32_t* keys, const int* rowptr, int n,
+                                long long vocab, const Slots& slots, void* out, float* parts, int width, int chunk, float scale, int accumulate,
+                                cudaStream_t st) {
   const int chunks = (n + chunk - 1) / chunk;
   constexpr int PER16 = 16 / sizeof(TI);
   const bool wide = width % PER16 == 0 && ld % PER16 == 0 && !(((uintptr_t)dy | (uintptr_t)out | (uintptr_t)parts) & 15);
-  const int vecs = wide ? width / PER16 : width;
+  const int per_thread = wide ? PER16 : 4;
+  const int vecs = (width + per_thread - 1) / per_thread;
   const int threads = vecs >= 256 ? 256 : (vecs + 31) / 32 * 32;
-  const dim3 grid(chunks, (vecs + threads - 1) / threads);
-  const size_t smem = (2 * chunk + 1) * sizeof(int);
+  const int fills = accumulate ? 0 : 148 * 2;
+  const dim3 grid(fills + chunks, (vecs + threads - 1) / threads);
+  const size_t smem = 2 * chunk * sizeof(int);
   cudaError_t e;
   if (wide) {
-    auto kern = embed_sum_kernel<TI, TO, PER16>;
-    e = launch_dependent(kern, grid, dim3(threads), smem, st, (const TI*)dy, ld, order, keys, rowptr, vocab, (TO*)out, parts, width, chunk,
-                         scale, accumulate);
+    auto kern = embed_sum_kernel<TI, TO, PER16, 1>;
+    e = launch_dependent(kern, grid, dim3(threads), smem, st, (const TI*)dy, ld, order, keys, rowptr, vocab, slots, (TO*)out, parts, width,
+                         chunk, fills, scale, accumulate);
   } else {
-    auto kern = embed_sum_kernel<TI, TO, 1>;
-    e = launch_dependent(kern, grid, dim3(threads), smem, st, (const TI*)dy, ld, order, keys, rowptr, vocab, (TO*)out, parts, width, chunk,
-                         scale, accumulate);
+    auto kern = embed_sum_kernel<TI, TO, 1, 4>;
+    e = launch_dependent(kern, grid, dim3(threads), smem, st, (const TI*)dy, ld, order, keys, rowptr, vocab, slots, (TO*)out, parts, width,
+                         chunk, fills, scale, accumulate);
   }
   if (e != cudaSuccess || chunks == 1) return e;
   auto kern = embed_join_kernel<TO>;
   return launch_dependent(kern, dim3(chunks - 1, (width + JOIN_COLS - 1) / JOIN_COLS), dim3(32 * JOIN_WARPS), 0, st, (const float*)parts, keys,
-                          rowptr, vocab, (TO*)out, width, chunk, scale, accumulate);
+                          rowptr, slots, (TO*)out, width, chunk, scale, accumulate);
 }
 
 template <typename ID>
-static cudaError_t sort_tokens(const void* ids, int n, long long vocab, long long padding, int* order, int* keys, int* rowptr, void* clear,
-                               long long row_bytes, cudaStream_t st) {
-  // one CTA per SM where the rows per CTA allow it, else two
-  const long long one = (vocab + 147) / 148, two = (vocab + 295) / 296;
-  const int rows_each = (int)(one <= SORT_ROWS ? one : two <= SORT_ROWS ? two : SORT_ROWS);
-  const size_t smem = (size_t)SORT_WARPS * rows_each * sizeof(int);
+static cudaError_t sort_tokens(const void* ids, int n, long long vocab, long long padding, const Slots& slots, int* order, uint32_t* keys,
+                               int* rowptr, cudaStream_t st) {
   auto kern = embed_sort_kernel<ID>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_WARPS * SORT_ROWS * (int)sizeof(int));
   if (e != cudaSuccess) return e;
-  return launch_dependent(kern, dim3((unsigned)((vocab + rows_each - 1) / rows_each)), dim3(SORT_WARPS * 32), smem, st, (const ID*)ids, n, vocab,
-                          padding, rows_each, order, keys, rowptr, (uint8_t*)clear, row_bytes);
+  return launch_dependent(kern, dim3(1u << slots.bits), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * slots.rows * sizeof(int), st, (const ID*)ids, n,
+                          vocab, padding, slots, order, keys, rowptr);
 }
 
 }  // namespace tnnb
@@ -352,12 +392,12 @@ int tnnb_embed_lookup(const void* ids, int ids64, const void* table, long long l
 }
 
 // out [vocab, width] (+)= scale * the sum of the rows of dy [n, width] (rows `ld` apart) per token. `out` has dy's type or is fp32;
-// without `accumulate` every row of it is written. Workspaces: `order` and `keys` int[n], `rowptr` int[vocab + 1], `parts`
+// without `accumulate` every row of it is written. Workspaces: `order` and `keys` int[n], `rowptr` int[vocab + vocab / 256 + 129], `parts`
 // float[2 * ceil(n / chunk) * width] on 16 bytes.
 int tnnb_embed_grad(const void* ids, int ids64, const void* dy, long long ld, void* out, void* order, void* keys, void* rowptr, void* parts,
                     int n, int width, long long vocab, long long padding, float scale, int type, int out_type, int accumulate, int chunk,
                     void* stream) {
-  if (n < 0 || width <= 0 || vocab <= 0 || vocab > 0x7ffffffe || ld < width || chunk < 1 || chunk > 1024) return -3;
+  if (n < 0 || width <= 0 || vocab <= 0 || vocab >= (1 << 30) || ld < width || chunk < 1 || chunk > 1024) return -3;
   if (out_type != VT_FP32 && (out_type != type || accumulate)) return -4;
   const cudaStream_t st = (cudaStream_t)stream;
   if (n == 0) {
@@ -365,15 +405,14 @@ int tnnb_embed_grad(const void* ids, int ids64, const void* dy, long long ld, vo
     const cudaError_t e = cudaMemsetAsync(out, 0, (size_t)vocab * width * value_size(out_type), st);
     return e == cudaSuccess ? 0 : -(int)e - 1000;
   }
-  void* clear = accumulate ? nullptr : out;
-  const long long row_bytes = (long long)width * value_size(out_type);
-  cudaError_t e = ids64 ? sort_tokens<long long>(ids, n, vocab, padding, (int*)order, (int*)keys, (int*)rowptr, clear, row_bytes, st)
-                        : sort_tokens<int>(ids, n, vocab, padding, (int*)order, (int*)keys, (int*)rowptr, clear, row_bytes, st);
+  const Slots slots = slots_of(vocab);
+  cudaError_t e = ids64 ? sort_tokens<long long>(ids, n, vocab, padding, slots, (int*)order, (uint32_t*)keys, (int*)rowptr, st)
+                        : sort_tokens<int>(ids, n, vocab, padding, slots, (int*)order, (uint32_t*)keys, (int*)rowptr, st);
   if (e != cudaSuccess) return -(int)e - 1000;
   const bool known = with_type(type, [&](auto tag) {
     using T = typename decltype(tag)::type;
     auto go = [&](auto to) {
-      return sum_and_join<T, typename decltype(to)::type>(dy, ld, (const int*)order, (const int*)keys, (const int*)rowptr, n, vocab, out,
+      return sum_and_join<T, typename decltype(to)::type>(dy, ld, (const int*)order, (const uint32_t*)keys, (const int*)rowptr, n, vocab, slots, out,
                                                           (float*)parts, width, chunk, scale, accumulate, st);
     };
     e = out_type == VT_FP32 ? go(TypeTag<float>()) : go(TypeTag<T>());

@@ -690,9 +690,11 @@ int tnnb_token_logprob(const void* z, long long ld, const void* tokens, int toke
   if (rows < 0 || V <= 0 || top < 0 || top > LP_TOP || top > V || (rows > 1 && ld < V)) return -3;
   if (rows * LP_CLUSTER > 0x7fffffffLL) return -3;
   if (rows == 0) return 0;
-  // Split rows while the SMs have room for more CTAs and a part still is a few vectors per thread.
+  // A CTA gets about 18 KB per us out of memory when it is alone on its SM; a cluster costs 2 us. Us with 1, 2, 4 and 8 CTAs per row:
+  // 8 x 50257 bf16 11.3, 10.6, 9.5, 10.1; 8 x 128001 fp32 19.9, 14.4, 11.2, 9.5; 20 x 20000 bf16 7.0, 8.1, 8.3, 8.5; 148 x 50257 9.7, 10.8, 13.8, 20.8.
   int parts = 1;
-  while (parts < LP_CLUSTER && rows * parts < 296 && V / (2 * parts) >= 4096) parts *= 2;
+  const long long bytes = (long long)V * (type == VT_FP32 ? 4 : 2);
+  while (parts < LP_CLUSTER && rows * parts * 2 <= 148 && bytes / parts >= 48 << 10) parts *= 2;
   const LogprobParams p = {z, ld, tokens, tokens64, rows, V, top, c, ignore, (float*)logp, (float*)entropy, (float*)top_logp,
                            (long long*)top_index, (float*)stats};
   cudaError_t e = cudaSuccess;

@@ -199,6 +199,8 @@ class _Embedding(torch.autograd.Function):
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * table[ids]`` (zeros at ``padding_idx``), shape ``[*ids.shape, width]``. The table's gradient adds each token's
     positions up in fp32, in an order that depends on the ids alone, and rounds once to the table's type."""
+    if not (table.requires_grad and torch.is_grad_enabled()):
+        return raw.embedding_lookup(ids, table, scale, padding_idx)
     return _Embedding.apply(ids, table, float(scale), padding_idx)
 
 

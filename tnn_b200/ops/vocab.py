@@ -21,8 +21,13 @@ _LOG2E = 1.4426950408889634
 _DECLARED = False
 
 
+_LIBRARY = None
+
+
 def _library():
-    global _DECLARED
+    global _DECLARED, _LIBRARY
+    if _LIBRARY is not None:
+        return _LIBRARY
     lib = _lib.load()
     if not _DECLARED:
         p, i, l, f = _lib.c_void_p, _lib.c_int, _lib.c_ll, _lib.c_float
@@ -31,6 +36,7 @@ def _library():
         _lib.declare(lib, "tnnb_token_logprob", [p, l, p, i, p, p, p, p, p, l, i, i, f, l, i, p])
         _lib.declare(lib, "tnnb_token_logprob_grad", [p, l, p, l, p, i, p, p, p, p, l, i, f, f, l, i, p])
         _DECLARED = True
+    _LIBRARY = lib
     return lib
 
 
@@ -42,17 +48,20 @@ def _type_code(t: torch.Tensor, what: str) -> int:
 
 
 def _whole(t: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
-    """Integer ids, flat and packed, on ``like``'s device."""
-    if t.dtype not in (torch.int64, torch.int32):
+    """Integer ids, packed, on ``like``'s device."""
+    if t.dtype is not torch.int64 and t.dtype is not torch.int32:
         raise TypeError(f"{what} is {t.dtype}; int64 or int32 expected")
     if t.device != like.device:
         raise ValueError(f"{what} is on {t.device}, not on {like.device}")
-    return t.reshape(-1).contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """``[rows, width]`` with a unit inner stride and rows that do not overlap."""
-    t = t.reshape(-1, width)
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    if t.is_contiguous():
+        return t
     return t if (t.stride(1) == 1 or width == 1) and (t.shape[0] < 2 or t.stride(0) >= width) else t.contiguous()
 
 
@@ -68,20 +77,22 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         raise ValueError(f"embedding table {tuple(table.shape)} of {table.dtype}: a floating-point matrix expected")
     rows, width = table.shape
     flat = _whole(ids, table, "ids")
-    if flat.numel() and (rows == 0 or width == 0):
+    n = flat.numel()
+    if n and (rows == 0 or width == 0):
         raise ValueError(f"embedding table {tuple(table.shape)} is empty")
     pad = _NO_PADDING if padding_idx is None else int(padding_idx)
     if table.is_cuda:
         code = _type_code(table, "embedding table")
         table = _rows(table, width)
         with _lib.device_of(table):
-            out = torch.empty(flat.numel(), width, dtype=table.dtype, device=table.device)
-            if flat.numel():
-                rc = _library().tnnb_embed_lookup(flat, int(flat.dtype == torch.int64), table, max(_pitch(table), width), out, flat.numel(),
-                                                  width, rows, pad, float(scale), code, _lib.raw_stream())
+            out = _lib.empty(table, *ids.shape, width)
+            if n:
+                rc = _library().tnnb_embed_lookup(flat, flat.dtype is torch.int64, table.data_ptr(), max(_pitch(table), width), out, n, width, rows, pad,
+                                                  float(scale), code, _lib.raw_stream())
                 _lib.check_rc(rc, "embedding_lookup")
                 LAUNCHES["count"] += 1
-        return out.view(*ids.shape, width)
+        return out
+    flat = flat.reshape(-1)
     safe = torch.where((flat < 0) | (flat >= rows), torch.zeros_like(flat), flat).long()
     wide = torch.promote_types(table.dtype, torch.float32)
     out = table[safe].to(wide) * scale
@@ -105,7 +116,7 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
     equal bits. ``out``: ``[rows, width]``, packed, of ``dy``'s type or fp32 (default: a new one of ``dy``'s type), every row of which
     is written; with ``accumulate`` (fp32) the sums are added to it instead."""
     rows = int(rows)
-    if dy.dim() < 1 or tuple(dy.shape[:-1]) != tuple(ids.shape) or not dy.is_floating_point():
+    if dy.dim() < 1 or dy.shape[:-1] != ids.shape or not dy.is_floating_point():
         raise ValueError(f"dy {tuple(dy.shape)} of {dy.dtype} does not belong to ids {tuple(ids.shape)}")
     width = dy.shape[-1]
     if rows <= 0 or width == 0:
@@ -126,20 +137,20 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
         code = _type_code(dy, "dy")
         dy2 = _rows(dy, width)
         with _lib.device_of(dy2):
-            dev = dy2.device
             if out is None:
-                out = torch.empty(rows, width, dtype=dy.dtype, device=dev)
+                out = _lib.empty(dy2, rows, width)
             chunk = _chunk(n)
             # sorted positions and their tokens, where each row's begin; partial sums of tokens in several chunks
-            ints = torch.empty(2 * n + rows + 1, dtype=torch.int32, device=dev)
-            parts = torch.empty(2 * ((n + chunk - 1) // chunk) * width, dtype=torch.float32, device=dev)
+            ints = _lib.empty(dy2, torch.int32, 2 * n + rows + rows // 256 + 129)
+            parts = _lib.empty(dy2, torch.float32, 2 * ((n + chunk - 1) // chunk) * width)
             base = ints.data_ptr()
-            rc = _library().tnnb_embed_grad(flat, int(flat.dtype == torch.int64), dy2, max(_pitch(dy2), width) if n else width, out, base,
+            rc = _library().tnnb_embed_grad(flat, flat.dtype is torch.int64, dy2, max(_pitch(dy2), width) if n else width, out, base,
                                             base + 4 * n, base + 8 * n, parts, n, width, rows, pad, float(scale), code, _TYPES[out.dtype],
                                             int(accumulate), chunk, _lib.raw_stream())
             _lib.check_rc(rc, "embedding_grad")
             LAUNCHES["count"] += 3 if n > chunk else 2
         return out
+    flat = flat.reshape(-1)
     safe = torch.where((flat < 0) | (flat >= rows), torch.zeros_like(flat), flat).long()
     g = dy.reshape(-1, width).to(torch.promote_types(dy.dtype, torch.float32))
     g = torch.where((flat == pad)[:, None], torch.zeros_like(g), g)
@@ -158,7 +169,7 @@ class TokenLogProbs(NamedTuple):
 
 
 def _check_rows(logits, tokens, top_k, temperature):
-    if logits.dim() < 1 or tuple(logits.shape[:-1]) != tuple(tokens.shape) or not logits.is_floating_point():
+    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape or not logits.is_floating_point():
         raise ValueError(f"logits {tuple(logits.shape)} of {logits.dtype} do not belong to tokens {tuple(tokens.shape)}")
     V = logits.shape[-1]
     if V == 0 or V >= 1 << 30:
@@ -179,26 +190,27 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
     the vocabulary has log probability NaN. A row with nothing but -inf has log probability -inf and entropy 0; a NaN or +inf logit
     makes a row's results NaN (NaN sorts first, and the indices are those of the largest logits all the same). ``keep``: a dict that
     receives what :func:`token_log_probs_grad` needs."""
-    V = _check_rows(logits, tokens, int(top_k), float(temperature))
-    top_k, temperature, shape = int(top_k), float(temperature), tuple(tokens.shape)
+    top_k, temperature, shape = int(top_k), float(temperature), tokens.shape
+    V = _check_rows(logits, tokens, top_k, temperature)
     tok = _whole(tokens, logits, "tokens")
     z = _rows(logits, V)
     rows = z.shape[0]
     if logits.is_cuda:
         code = _type_code(logits, "logits")
         with _lib.device_of(z):
-            dev, f32 = z.device, torch.float32
-            lp, ent = torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev)
-            top, idx = torch.empty(rows, top_k, dtype=f32, device=dev), torch.empty(rows, top_k, dtype=torch.int64, device=dev)
-            stats = torch.empty(rows, 2, dtype=f32, device=dev) if keep is not None else None
+            f32 = torch.float32
+            lp, ent = _lib.empty(z, f32, *shape), _lib.empty(z, f32, *shape)
+            top, idx = _lib.empty(z, f32, *shape, top_k), _lib.empty(z, torch.int64, *shape, top_k)
+            stats = _lib.empty(z, f32, rows, 2) if keep is not None else None
             if rows:
-                rc = _library().tnnb_token_logprob(z, max(_pitch(z), V), tok, int(tok.dtype == torch.int64), lp, ent, top, idx, stats, rows, V,
-                                                   top_k, _LOG2E / temperature, int(ignore_index), code, _lib.raw_stream())
+                rc = _library().tnnb_token_logprob(z.data_ptr(), max(_pitch(z), V), tok, tok.dtype is torch.int64, lp, ent, top, idx, stats, rows, V, top_k,
+                                                   _LOG2E / temperature, int(ignore_index), code, _lib.raw_stream())
                 _lib.check_rc(rc, "token_log_probs")
                 LAUNCHES["count"] += 1
         if keep is not None:
             keep.update(stats=stats, entropy=ent)
-        return TokenLogProbs(lp.view(shape), ent.view(shape), top.view(*shape, top_k), idx.view(*shape, top_k))
+        return TokenLogProbs(lp, ent, top, idx)
+    tok = tok.reshape(-1)
     wide = torch.promote_types(z.dtype, torch.float32)
     zf = z.to(wide)
     logp, p, plogp = _distribution(zf, temperature)
@@ -251,14 +263,17 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
         code = _type_code(logits, "logits")
         with _lib.device_of(z):
             pitch = max(_pitch(z), V)
-            dz = torch.empty(rows, pitch, dtype=z.dtype, device=z.device)[:, :V]
+            dz = _lib.empty(z, rows, pitch)
+            if pitch != V:
+                dz = dz[:, :V]
             if rows:
-                rc = _library().tnnb_token_logprob_grad(z, pitch, dz, pitch, tok, int(tok.dtype == torch.int64), kept["stats"], kept["entropy"],
+                rc = _library().tnnb_token_logprob_grad(z.data_ptr(), pitch, dz, pitch, tok, tok.dtype is torch.int64, kept["stats"], kept["entropy"],
                                                         g, h, rows, V, _LOG2E / float(temperature), 1.0 / float(temperature),
                                                         int(ignore_index), code, _lib.raw_stream())
                 _lib.check_rc(rc, "token_log_probs_grad")
                 LAUNCHES["count"] += 1
         return dz.view(logits.shape) if pitch == V else dz.unflatten(0, logits.shape[:-1])
+    tok = tok.reshape(-1)
     zf = z.to(torch.promote_types(z.dtype, torch.float32))
     logp, p, plogp = _distribution(zf, float(temperature))
     dead = torch.isneginf(zf).all(1)
