@@ -73,7 +73,7 @@ const Entry SIGNATURES[] = {
     SIG("pplifp"), SIG("ppplifp"), SIG("pppliip"),      // act_fwd, act_bwd, binary
     SIG("pplfupp"),                                     // dropout
     SIG("ppppliillfupp"),                               // embedding_fwd, embedding_bwd
-    SIG("piplplillfip"), SIG("piplppppp" "iillfiiiip"),  // embed_lookup, embed_grad
+    SIG("piplplillfip"), SIG("piplpppppp" "iillfiiiip"),  // embed_lookup, embed_grad
     SIG("plpipppppliiflip"), SIG("plplpipppp" "liffl" "ip"),  // token_logprob, token_logprob_grad
     SIG("plliiiipif" "pppppppppp"),  // newton_schulz
     SIG("plplip"), SIG("pplp"), SIG("plpplip"),         // colsum_accum, cast_f32_bf16, scale_by

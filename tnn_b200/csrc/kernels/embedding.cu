@@ -6,8 +6,8 @@
 // bf16, fp16 and fp32, any width; ids of 32 or 64 bits. Products and sums are fp32, rounded once. An id outside the table reads
 // (and adds to) row 0 like the layers' embedding kernels (elementwise.cu); the bounds-checked build records it.
 //
-// The gradient adds up in a fixed order: the positions of each token ascending, in chunks of the sorted list, then the chunks
-// ascending. No atomics on values: the same inputs give the same bits, and a row is written once, in the table's own type.
+// The gradient adds up in an order that depends on the ids alone: the positions of each token as sorted, in chunks of the sorted list,
+// then the chunks. No atomics on values: the same inputs give the same bits, and a row is written once, in the table's own type.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "values.cuh"
@@ -53,7 +53,7 @@ embed_lookup_kernel(const ID* __restrict__ ids, const T* __restrict__ table, lon
 }
 
 // -------------------------------------------------------------------------------------------------------------- sort
-// Positions sorted by token, stable, without a pass over global counters: every CTA owns some table rows, reads ALL ids (they come
+// Positions sorted by token, in an order that depends on the ids alone, without a pass over global counters: every CTA owns some table rows, reads ALL ids (they come
 // from L2: 64 KB for 8192 tokens) and picks its own. The number of ids that belong to CTAs before it is the place of its part of
 // the list, so no CTA waits for another. Within the CTA each warp walks a contiguous stretch of the ids and has a counter per row:
 // counts, then starting places (rows ascending, warps ascending within a row), then the places themselves. A place gets its token with
@@ -63,7 +63,7 @@ embed_lookup_kernel(const ID* __restrict__ ids, const T* __restrict__ table, lon
 // with ranges of rows the CTA that had them took 16 us for 8192 tokens of text, 63 for 50001. The list is in this order of rows
 // ("slots"), which is as good as any.
 static constexpr int SORT_WARPS = 32;
-static constexpr int SORT_ROWS = 512;  // most rows of a CTA: 64 KB of counters, two CTAs per SM
+static constexpr int SORT_ROWS = 512;  // most rows of a CTA, one per thread
 static constexpr uint32_t TOKEN_FIRST = 1u << 30, TOKEN_LAST = 1u << 31, TOKEN_ROW = TOKEN_FIRST - 1;
 
 struct Slots {
@@ -79,62 +79,84 @@ __host__ __device__ __forceinline__ Slots slots_of(long long vocab) {
 }
 __device__ __forceinline__ int slot_of(const Slots& s, int row) { return (row & ((1 << s.bits) - 1)) * s.rows + (row >> s.bits); }
 
+// A position's CTA and the row's number there, 16 bits each (NO_CODE: padding). Every CTA looks at every position twice: what it
+// does to an id is done once, here, and four instructions are left (200000 positions: 28 us per look with the ids themselves).
+static constexpr uint32_t NO_CODE = 0xffffffffu;
 template <typename ID>
-__device__ __forceinline__ int sort_row(const ID* ids, int i, long long vocab, long long padding) {
-  const long long id = ids[i];
-  if (id == padding) return -1;
-  (void)TNNB_CHECK(id, vocab);
-  return id < 0 || id >= vocab ? 0 : (int)id;
-}
-
-template <typename ID>
-__global__ void __launch_bounds__(SORT_WARPS * 32)
-embed_sort_kernel(const ID* ids, int n, long long vocab, long long padding, Slots slots, int* order, uint32_t* keys, int* rowptr) {
+__global__ void __launch_bounds__(256)
+embed_code_kernel(const ID* ids, int n, long long vocab, long long padding, Slots slots, uint32_t* codes) {
   grid_dep_launch();
   grid_dep_wait();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  long long id = ids[i];
+  const bool pad = id == padding;
+  if (!pad) (void)TNNB_CHECK(id, vocab);
+  if (id < 0 || id >= vocab) id = 0;
+  codes[i] = pad ? NO_CODE : (uint32_t)(id & ((1 << slots.bits) - 1)) << 16 | (uint32_t)(id >> slots.bits);
+}
+
+__global__ void __launch_bounds__(SORT_WARPS * 32)
+embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_t* keys, int* rowptr) {
   extern __shared__ int counters[];  // [SORT_WARPS][slots.rows]
   __shared__ int below[SORT_WARPS], scan[SORT_WARPS];
   __shared__ int begin[SORT_ROWS], count[SORT_ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = slots.rows, own = blockIdx.x, mask = (1 << slots.bits) - 1;
   for (int i = threadIdx.x; i < SORT_WARPS * rows; i += blockDim.x) counters[i] = 0;
+  grid_dep_launch();
+  grid_dep_wait();
   __syncthreads();
 
-  const int stretch = ((n + SORT_WARPS - 1) / SORT_WARPS + 31) / 32 * 32;
+  const int stretch = ((n + SORT_WARPS - 1) / SORT_WARPS + 127) / 128 * 128;  // of a warp
   const int lo = min((long long)n, (long long)warp * stretch), hi = min((long long)n, (long long)lo + stretch);
   int* mine = counters + warp * rows;
-  int less = 0;
-  constexpr int AHEAD = 8;
-  for (int i0 = lo; i0 < hi; i0 += 32 * AHEAD) {
-    int r[AHEAD];
+  const uint32_t base = (uint32_t)own << 16;
+  // Calls f(four codes, place of the first) for the warp's positions, 128 at a time; the next ones are on their way meanwhile. (`codes`
+  // begins on 16 bytes and ends on a whole vector.)
+  auto walk = [&](auto f) {
+    constexpr int SETS = 2;
+    uint4 now[SETS], next[SETS];
+    auto load = [&](int i0, uint4 (&v)[SETS]) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) r[u] = i0 + u * 32 + lane < hi ? sort_row(ids, i0 + u * 32 + lane, vocab, padding) : -1;
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      less += r[u] >= 0 && (r[u] & mask) < own;
-      const bool in = r[u] >= 0 && (r[u] & mask) == own;
-      const unsigned who = __ballot_sync(0xffffffffu, in);
-      if (who == 0) continue;
-      if (in) {
-        const int at = r[u] >> slots.bits;
-        const unsigned same = __match_any_sync(who, at);
-        if ((same & ((1u << lane) - 1)) == 0) mine[at] += __popc(same);
+      for (int h = 0; h < SETS; ++h) {
+        const int i = i0 + h * 128 + lane * 4;
+        v[h] = i < hi ? *reinterpret_cast<const uint4*>(codes + i) : make_uint4(NO_CODE, NO_CODE, NO_CODE, NO_CODE);
       }
-      __syncwarp();
+    };
+    load(lo, now);
+    for (int i0 = lo; i0 < hi; i0 += 128 * SETS) {
+      load(i0 + 128 * SETS, next);
+#pragma unroll
+      for (int h = 0; h < SETS; ++h) {
+        const int i = i0 + h * 128 + lane * 4;
+        const uint32_t w[4] = {now[h].x, i + 1 < hi ? now[h].y : NO_CODE, i + 2 < hi ? now[h].z : NO_CODE, i + 3 < hi ? now[h].w : NO_CODE};
+        f(w, i);
+        now[h] = next[h];
+      }
     }
-  }
+  };
+  int less = 0;
+  walk([&](const uint32_t (&w)[4], int) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      less += w[j] < base;
+      if (w[j] - base < 65536u) atomicAdd(&mine[w[j] & 0xffffu], 1);
+    }
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) less += __shfl_xor_sync(0xffffffffu, less, o);
   if (lane == 0) below[warp] = less;
   __syncthreads();
 
-  int total = 0;
-  if ((int)threadIdx.x < rows)
-    for (int w = 0; w < SORT_WARPS; ++w) {
-      const int c = counters[w * rows + threadIdx.x];
-      counters[w * rows + threadIdx.x] = total;
-      total += c;
-    }
+  int total = 0, c[SORT_WARPS];
+  const int row = threadIdx.x;
+  if (row < rows) {
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; ++w) c[w] = counters[w * rows + row];
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; ++w) total += c[w];
+  }
   int upto = total;  // sum over the rows up to this thread's
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -144,38 +166,45 @@ embed_sort_kernel(const ID* ids, int n, long long vocab, long long padding, Slot
   if (lane == 31) scan[warp] = upto;
   __syncthreads();
   int start = upto - total;
+#pragma unroll
   for (int w = 0; w < SORT_WARPS; ++w) start += below[w] + (w < warp ? scan[w] : 0);
-  if ((int)threadIdx.x < rows) {
-    rowptr[own * rows + threadIdx.x] = start;
-    if (own == mask && (int)threadIdx.x == rows - 1) rowptr[(mask + 1) * rows] = start + total;
-    for (int w = 0; w < SORT_WARPS; ++w) counters[w * rows + threadIdx.x] += start;
-    begin[threadIdx.x] = start, count[threadIdx.x] = total;
+  if (row < rows) {
+    rowptr[own * rows + row] = start;
+    if (own == mask && row == rows - 1) rowptr[(mask + 1) * rows] = start + total;
+    begin[row] = start, count[row] = total;
+    int at = start;
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; ++w) {
+      counters[w * rows + row] = at;
+      at += c[w];
+    }
   }
   __syncthreads();
 
-  for (int i0 = lo; i0 < hi; i0 += 32 * AHEAD) {
-    int r[AHEAD];
+  walk([&](const uint32_t (&w)[4], int position) {
+    bool any = false;
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) r[u] = i0 + u * 32 + lane < hi ? sort_row(ids, i0 + u * 32 + lane, vocab, padding) : -1;
+    for (int j = 0; j < 4; ++j) any |= w[j] - base < 65536u;
+    if (!__any_sync(0xffffffffu, any)) return;
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const bool in = r[u] >= 0 && (r[u] & mask) == own;
+    for (int j = 0; j < 4; ++j) {
+      const bool in = w[j] - base < 65536u;
       const unsigned who = __ballot_sync(0xffffffffu, in);
       if (who == 0) continue;
-      int at = 0;
-      unsigned same = 0;
       if (in) {
-        at = r[u] >> slots.bits;
-        same = __match_any_sync(who, at);
+        const int at = w[j] & 0xffffu;
+        // lanes with the same row, in their order
+        const unsigned same = (who & (who - 1)) ? __match_any_sync(who, at) : who;
         const int to = mine[at] + __popc(same & ((1u << lane) - 1));
-        order[to] = i0 + u * 32 + lane;
-        keys[to] = (uint32_t)r[u] | (to == begin[at] ? TOKEN_FIRST : 0u) | (to + 1 == begin[at] + count[at] ? TOKEN_LAST : 0u);
+        order[to] = position + j;
+        keys[to] = ((uint32_t)at << slots.bits | (uint32_t)own) | (to == begin[at] ? TOKEN_FIRST : 0u) |
+                   (to + 1 == begin[at] + count[at] ? TOKEN_LAST : 0u);
+        __syncwarp(same);
+        if ((same & ((1u << lane) - 1)) == 0) mine[at] = to + __popc(same);
       }
       __syncwarp();
-      if (in && (same & ((1u << lane) - 1)) == 0) mine[at] += __popc(same);
-      __syncwarp();
     }
-  }
+  });
 }
 
 // -------------------------------------------------------------------------------------------------------------- sums
@@ -347,13 +376,15 @@ static cudaError_t sum_and_join(const void* dy, long long ld, const int* order, 
 }
 
 template <typename ID>
-static cudaError_t sort_tokens(const void* ids, int n, long long vocab, long long padding, const Slots& slots, int* order, uint32_t* keys,
-                               int* rowptr, cudaStream_t st) {
-  auto kern = embed_sort_kernel<ID>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_WARPS * SORT_ROWS * (int)sizeof(int));
+static cudaError_t sort_tokens(const void* ids, int n, long long vocab, long long padding, const Slots& slots, uint32_t* codes, int* order,
+                               uint32_t* keys, int* rowptr, cudaStream_t st) {
+  auto code = embed_code_kernel<ID>;
+  cudaError_t e = launch_dependent(code, dim3((n + 255) / 256), dim3(256), 0, st, (const ID*)ids, n, vocab, padding, slots, codes);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kern, dim3(1u << slots.bits), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * slots.rows * sizeof(int), st, (const ID*)ids, n,
-                          vocab, padding, slots, order, keys, rowptr);
+  e = cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_WARPS * SORT_ROWS * (int)sizeof(int));
+  if (e != cudaSuccess) return e;
+  return launch_dependent(embed_sort_kernel, dim3(1u << slots.bits), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * slots.rows * sizeof(int), st,
+                          (const uint32_t*)codes, n, slots, order, keys, rowptr);
 }
 
 }  // namespace tnnb
@@ -392,12 +423,12 @@ int tnnb_embed_lookup(const void* ids, int ids64, const void* table, long long l
 }
 
 // out [vocab, width] (+)= scale * the sum of the rows of dy [n, width] (rows `ld` apart) per token. `out` has dy's type or is fp32;
-// without `accumulate` every row of it is written. Workspaces: `order` and `keys` int[n], `rowptr` int[vocab + vocab / 256 + 129], `parts`
-// float[2 * ceil(n / chunk) * width] on 16 bytes.
-int tnnb_embed_grad(const void* ids, int ids64, const void* dy, long long ld, void* out, void* order, void* keys, void* rowptr, void* parts,
-                    int n, int width, long long vocab, long long padding, float scale, int type, int out_type, int accumulate, int chunk,
+// without `accumulate` every row of it is written. Workspaces: `codes` uint32[n rounded up to 4] on 16 bytes, `order` and `keys` int[n],
+// `rowptr` int[vocab + vocab / 256 + 129], `parts` float[2 * ceil(n / chunk) * width] on 16 bytes.
+int tnnb_embed_grad(const void* ids, int ids64, const void* dy, long long ld, void* out, void* codes, void* order, void* keys, void* rowptr,
+                    void* parts, int n, int width, long long vocab, long long padding, float scale, int type, int out_type, int accumulate, int chunk,
                     void* stream) {
-  if (n < 0 || width <= 0 || vocab <= 0 || vocab >= (1 << 30) || ld < width || chunk < 1 || chunk > 1024) return -3;
+  if (n < 0 || width <= 0 || vocab <= 0 || vocab > (1 << 24) || ld < width || chunk < 1 || chunk > 1024) return -3;
   if (out_type != VT_FP32 && (out_type != type || accumulate)) return -4;
   const cudaStream_t st = (cudaStream_t)stream;
   if (n == 0) {
@@ -406,8 +437,8 @@ int tnnb_embed_grad(const void* ids, int ids64, const void* dy, long long ld, vo
     return e == cudaSuccess ? 0 : -(int)e - 1000;
   }
   const Slots slots = slots_of(vocab);
-  cudaError_t e = ids64 ? sort_tokens<long long>(ids, n, vocab, padding, slots, (int*)order, (uint32_t*)keys, (int*)rowptr, st)
-                        : sort_tokens<int>(ids, n, vocab, padding, slots, (int*)order, (uint32_t*)keys, (int*)rowptr, st);
+  cudaError_t e = ids64 ? sort_tokens<long long>(ids, n, vocab, padding, slots, (uint32_t*)codes, (int*)order, (uint32_t*)keys, (int*)rowptr, st)
+                        : sort_tokens<int>(ids, n, vocab, padding, slots, (uint32_t*)codes, (int*)order, (uint32_t*)keys, (int*)rowptr, st);
   if (e != cudaSuccess) return -(int)e - 1000;
   const bool known = with_type(type, [&](auto tag) {
     using T = typename decltype(tag)::type;

@@ -32,7 +32,7 @@ def _library():
     if not _DECLARED:
         p, i, l, f = _lib.c_void_p, _lib.c_int, _lib.c_ll, _lib.c_float
         _lib.declare(lib, "tnnb_embed_lookup", [p, i, p, l, p, l, i, l, l, f, i, p])
-        _lib.declare(lib, "tnnb_embed_grad", [p, i, p, l, p, p, p, p, p, i, i, l, l, f, i, i, i, i, p])
+        _lib.declare(lib, "tnnb_embed_grad", [p, i, p, l, p, p, p, p, p, p, i, i, l, l, f, i, i, i, i, p])
         _lib.declare(lib, "tnnb_token_logprob", [p, l, p, i, p, p, p, p, p, l, i, i, f, l, i, p])
         _lib.declare(lib, "tnnb_token_logprob_grad", [p, l, p, l, p, i, p, p, p, p, l, i, f, f, l, i, p])
         _DECLARED = True
@@ -123,8 +123,8 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
         raise ValueError(f"the gradient of a table of {rows} rows of {width} elements is empty")
     flat = _whole(ids, dy, "ids")
     n = flat.numel()
-    if n >= 1 << 30 or rows >= 1 << 30:
-        raise ValueError(f"{n} positions and {rows} rows: fewer than 2^30 of each are supported")
+    if n >= 1 << 30 or rows > 1 << 24:
+        raise ValueError(f"{n} positions and {rows} rows: fewer than 2^30 and at most 2^24 are supported")
     if accumulate and out is None:
         raise ValueError("accumulate needs an output to add to")
     if out is not None:
@@ -140,15 +140,16 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
             if out is None:
                 out = _lib.empty(dy2, rows, width)
             chunk = _chunk(n)
-            # sorted positions and their tokens, where each row's begin; partial sums of tokens in several chunks
-            ints = _lib.empty(dy2, torch.int32, 2 * n + rows + rows // 256 + 129)
+            # where each position belongs, sorted positions and their tokens, where each row's begin; partial sums of tokens in several chunks
+            n4 = (n + 3) // 4 * 4
+            ints = _lib.empty(dy2, torch.int32, n4 + 2 * n + rows + rows // 256 + 129)
             parts = _lib.empty(dy2, torch.float32, 2 * ((n + chunk - 1) // chunk) * width)
             base = ints.data_ptr()
             rc = _library().tnnb_embed_grad(flat, flat.dtype is torch.int64, dy2, max(_pitch(dy2), width) if n else width, out, base,
-                                            base + 4 * n, base + 8 * n, parts, n, width, rows, pad, float(scale), code, _TYPES[out.dtype],
+                                            base + 4 * n4, base + 4 * (n4 + n), base + 4 * (n4 + 2 * n), parts, n, width, rows, pad, float(scale), code, _TYPES[out.dtype],
                                             int(accumulate), chunk, _lib.raw_stream())
             _lib.check_rc(rc, "embedding_grad")
-            LAUNCHES["count"] += 3 if n > chunk else 2
+            LAUNCHES["count"] += 4 if n > chunk else 3
         return out
     flat = flat.reshape(-1)
     safe = torch.where((flat < 0) | (flat >= rows), torch.zeros_like(flat), flat).long()
