@@ -3,6 +3,7 @@
     train     --config x.json [--layout dp8|tp2dp4|pp2 ...]   single device, or one rank of a torchrun job
     infer     --config x.json                                  validation loss / accuracy of model_path or a fresh model
     generate  --model gpt2_small|--model-path f.tnng --vocab vocab.bin [--tokens train.bin]
+    score     --model gpt2_small|--model-path f.tnng --token-ids 1,2,3|--tokens train.bin [--top k]   log probabilities, perplexity
     tcp-worker      [port] [--host H] [--gpu]                  one pipeline stage served over TCP
     tcp-coordinator --config x.json                            partition a model, deploy it to TCP workers, train
     info                                                       devices, build status, registered models and layers
@@ -109,6 +110,37 @@ def cmd_generate(a) -> int:
     out = greedy_generate(g, prompt, a.num_tokens, eos=a.eos, seq_len=a.seq_len or model_seq_len(g),
                           on_token=lambda t: print(show([t]), end=" " if not tok else "", flush=True))
     print("\n\n[FULL TEXT]:\n" + show(out))
+    return 0
+
+
+def cmd_score(a) -> int:
+    """Log probabilities of a text's tokens, with each one's alternatives, and the text's perplexity."""
+    import math
+
+    from .data.tokenizer import Tokenizer
+    from .inference import score_tokens
+    from .models import zoo
+    from .nn.graph import Graph
+
+    dev = torch.device("cuda" if (a.device.upper() == "CUDA" and torch.cuda.is_available()) else "cpu")
+    g = Graph.load_state(a.model_path, device=dev) if a.model_path else zoo.create(a.model).compile(device=dev, seed=a.seed)
+    if a.token_ids:
+        ids = [int(t) for t in a.token_ids.split(",")]
+    elif a.tokens:
+        import numpy as np
+
+        ids = [int(t) for t in np.memmap(a.tokens, dtype=np.uint16, mode="r")[:a.max_tokens]]
+    else:
+        raise SystemExit("score needs --token-ids or --tokens")
+    tok = Tokenizer(a.vocab) if a.vocab else None
+    show = (lambda t: repr(tok.decode([t]))) if tok else str
+    r = score_tokens(g, ids, a.top, a.temperature, a.seq_len or None)
+    lp, ent, top, idx = (t.tolist() for t in r)
+    if not a.quiet:
+        for t, l, h, ps, ts in zip(ids[1:], lp, ent, top, idx):
+            print(f"{show(t)}  {l:.4f}  entropy {h:.4f}" + "".join(f"  {show(i)} {p:.4f}" for i, p in zip(ts, ps)))
+    mean = sum(lp) / len(lp)
+    print(json.dumps({"tokens": len(lp), "mean_log_prob": mean, "perplexity": math.exp(min(-mean, 80.0)), "mean_entropy": sum(ent) / len(ent)}))
     return 0
 
 
@@ -219,6 +251,19 @@ def main(argv=None) -> int:
     p.add_argument("--eos", type=int, default=50256)
     p.add_argument("--device", default=default_device_type(), help="CPU or CUDA (default: $DEVICE_TYPE, else CUDA when present)")
     p.add_argument("--seed", type=int, default=0)
+    p = sub.add_parser("score", help="log probabilities and perplexity of a text under a language model")
+    p.add_argument("--model", default="gpt2_small")
+    p.add_argument("--model-path", default="")
+    p.add_argument("--vocab", default="")
+    p.add_argument("--tokens", default="", help="uint16 token file to score the beginning of")
+    p.add_argument("--max-tokens", type=int, default=4096)
+    p.add_argument("--token-ids", default="", help="comma separated token ids")
+    p.add_argument("--top", type=int, default=0, help="most likely tokens to show beside each (up to 32)")
+    p.add_argument("--temperature", type=float, default=1.0)
+    p.add_argument("--seq-len", type=int, default=0)
+    p.add_argument("--quiet", action="store_true", help="print the summary only")
+    p.add_argument("--device", default=default_device_type(), help="CPU or CUDA (default: $DEVICE_TYPE, else CUDA when present)")
+    p.add_argument("--seed", type=int, default=0)
     p = sub.add_parser("tcp-worker", help="serve one pipeline stage over TCP until the coordinator shuts it down")
     p.add_argument("port", type=int, nargs="?", default=0)
     p.add_argument("--host", default="127.0.0.1")
@@ -230,7 +275,7 @@ def main(argv=None) -> int:
     p.add_argument("--val-batches", type=int, default=4, help="validation batches after training (0 = none)")
     sub.add_parser("info", help="build and device information")
     a = ap.parse_args(argv)
-    return {"train": cmd_train, "infer": cmd_infer, "generate": cmd_generate, "info": cmd_info,
+    return {"train": cmd_train, "infer": cmd_infer, "generate": cmd_generate, "score": cmd_score, "info": cmd_info,
             "tcp-worker": cmd_tcp_worker, "tcp-coordinator": cmd_tcp_coordinator}[a.cmd](a)
 
 

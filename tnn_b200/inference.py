@@ -1,4 +1,4 @@
-"""Inference helpers: validation of a saved or fresh model and greedy text generation.
+"""Inference helpers: validation of a saved or fresh model, greedy text generation and the scoring of texts.
 
 Reference: examples/inferencer.cpp:12-70 (validation loss / accuracy from ``model_path`` or a fresh zoo
 model) and examples/gpt2_inference.cpp:16-114 (greedy decoding: the prompt is right-padded with zeros to
@@ -15,6 +15,7 @@ from .nn.blocks import FlashAttentionBlock
 from .nn.graph import Graph
 from .nn.layers import (Add, Dense, Div, Dropout, ELU, Embedding, GELU, LayerNorm, LeakyReLU, Mul, PositionalEmbedding, ReLU,
                         Sigmoid, Sub, Tanh)
+from .ops import raw
 
 _PER_POSITION = (Add, Dense, Div, Dropout, ELU, Embedding, GELU, LayerNorm, LeakyReLU, Mul, ReLU, Sigmoid, Sub, Tanh)
 
@@ -83,6 +84,48 @@ def greedy_generate(graph: Graph, prompt: Iterable[int], num_new: int = 50, eos:
     finally:
         graph.set_training(was_training)
     return tokens
+
+
+@torch.no_grad()
+def score_tokens(graph: Graph, tokens: Iterable[int], top_k: int = 0, temperature: float = 1.0, seq_len: Optional[int] = None,
+                 context: Optional[int] = None, batch: int = 8) -> raw.TokenLogProbs:
+    """Log probability of every token of a text behind its first under a language model, with the entropies of the distributions they
+    were drawn from and their ``top_k`` most likely tokens (:func:`raw.token_log_probs`); entry ``i`` belongs to ``tokens[i + 1]``.
+
+    A text longer than the model's sequence length (``seq_len``) is read in windows, ``batch`` at a time, each of which repeats the last ``context``
+    tokens of the one before (default: half a window), so that no token is judged from fewer, except at the beginning."""
+    ids = torch.tensor([int(t) for t in tokens], dtype=torch.long)
+    n = ids.numel()
+    if n < 2:
+        raise ValueError(f"a text of {n} tokens has none behind its first")
+    S = seq_len or model_seq_len(graph) or n
+    context = S // 2 if context is None else int(context)
+    if not 0 <= context < S or batch < 1:
+        raise ValueError(f"a context of {context} tokens in windows of {S}, {batch} at a time")
+    # window w predicts the tokens behind positions starts[w] + skips[w] .. starts[w] + S - 1
+    starts, skips = [0], [0]
+    while starts[-1] + S < n - 1:
+        starts.append(starts[-1] + S - context)
+        skips.append(context)
+    was_training = graph.training
+    graph.set_training(False)
+    parts = []
+    try:
+        for w0 in range(0, len(starts), batch):
+            some = starts[w0:w0 + batch]
+            x, y = torch.zeros(len(some), S, dtype=torch.long), torch.full((len(some), S), -100, dtype=torch.long)
+            for r, (s, skip) in enumerate(zip(some, skips[w0:w0 + batch])):
+                have = min(S, n - s)
+                x[r, :have] = ids[s:s + have]
+                known = min(S, n - 1 - s)
+                y[r, skip:known] = ids[s + 1 + skip:s + 1 + known]
+            logits = graph.forward({graph.input_nodes[0].uid(): x.to(graph.device)})[graph.output_nodes[0].uid()]
+            r = raw.token_log_probs(logits, y.to(graph.device), top_k, temperature)
+            keep = (y != -100).reshape(-1).nonzero()[:, 0].to(graph.device)
+            parts.append([t.flatten(0, 1).index_select(0, keep) for t in r])
+    finally:
+        graph.set_training(was_training)
+    return raw.TokenLogProbs(*(torch.cat(c) for c in zip(*parts)))
 
 
 @torch.no_grad()

@@ -189,6 +189,97 @@ class AdamW(Adam):
         super().__init__(learning_rate, beta1, beta2, epsilon, weight_decay, True)
 
 
+class Muon(Optimizer):
+    """Momentum whose update is orthogonalised for weight matrices, AdamW for everything else.
+
+    Every dense, attention and convolution weight is a matrix ``[outputs, inputs]`` (a filter ``[O, KH, KW, I]`` as
+    ``[O, KH * KW * I]``): ``buffer = mu * buffer + (1 - mu) * g``, Nesterov's mix of buffer and gradient, five Newton-Schulz steps
+    (:func:`raw.newton_schulz`, all equal matrices of the model at once), ``w -= lr * (scale * update + weight_decay * w)`` with
+    ``scale = max(1, outputs / inputs) ** 0.5``. Embeddings, the layer that makes the graph's output, norms and biases take AdamW
+    with ``adam_learning_rate`` (schedulers move both rates in proportion). The reference has no such optimizer."""
+    TYPE = "muon"
+    PIECE = 4096  # elements of the other parameters per block of the AdamW launch
+
+    def __init__(self, learning_rate: float = 0.02, momentum: float = 0.95, nesterov: bool = True, ns_steps: int = 5,
+                 weight_decay: float = 0.0, adam_learning_rate: float = 3e-4, beta1: float = 0.9, beta2: float = 0.95, epsilon: float = 1e-8,
+                 adam_weight_decay: float = 0.0):
+        super().__init__(learning_rate)
+        if not (self.lr > 0 and adam_learning_rate > 0 and 0 <= momentum < 1 and 1 <= int(ns_steps) <= 64):
+            raise ValueError(f"muon: learning rates {learning_rate}, {adam_learning_rate}, momentum {momentum}, {ns_steps} steps")
+        self.momentum, self.nesterov, self.ns_steps = float(momentum), bool(nesterov), int(ns_steps)
+        self.weight_decay, self.adam_weight_decay = float(weight_decay), float(adam_weight_decay)
+        self.ratio = float(adam_learning_rate) / self.lr
+        self.beta1, self.beta2, self.eps = float(beta1), float(beta2), float(epsilon)
+        self.groups: List[raw.MatrixGroup] = []
+        self.buffer: Optional[torch.Tensor] = None  # momentum of all matrices, group after group
+        self.m: Optional[torch.Tensor] = None       # moments of the other parameters
+        self.v: Optional[torch.Tensor] = None
+
+    def attach(self, graph) -> "Muon":
+        from .layers import ClassToken, Embedding, PositionalEmbedding
+
+        self.graph = graph
+        dev = graph.master_flat.device
+        outputs = {id(n) for n in graph.output_nodes}
+        last = {id(e.layer) for e in graph.edges if any(id(c) in outputs for c in e.consumers)}
+        shapes: Dict[tuple, List[int]] = {}
+        rest = []
+        for layer in graph.layers():
+            for (off, n, shape, trainable), spec in zip(graph.layer_slices[id(layer)], layer.param_specs()):
+                if not trainable:
+                    continue
+                if len(shape) >= 2 and id(layer) not in last and not isinstance(layer, (Embedding, PositionalEmbedding, ClassToken)):
+                    if spec.sharded:
+                        raise ValueError(f"muon orthogonalises whole matrices: {layer.name}.{spec.name} is one shard of a tensor-parallel layer")
+                    shapes.setdefault((shape[0], n // shape[0]), []).append(off)
+                else:
+                    rest.append((off, n))
+        self.groups = [raw.MatrixGroup(m, n, offs, dev) for (m, n), offs in sorted(shapes.items())]
+        self.buffer = torch.zeros(sum(g.size * len(g.offsets) for g in self.groups), dtype=torch.float32, device=dev)
+        pieces, at = [], 0
+        for off, n in rest:
+            for k in range(0, n, self.PIECE):
+                pieces.append((off + k, min(self.PIECE, n - k), at + k))
+            at += n
+        self.pieces = torch.tensor(pieces, dtype=torch.int64, device=dev).reshape(-1, 3)
+        self.m = torch.zeros(at, dtype=torch.float32, device=dev)
+        self.v = torch.zeros_like(self.m)
+        return self
+
+    def prepare_step(self):
+        super().prepare_step()
+        if self.hyper is not None:
+            self._push_hyper(self.lr, 1 - self.beta1 ** self.step_count, 1 - self.beta2 ** self.step_count, self.grad_scale)
+
+    def update(self, prepared: bool = False, sl=None):
+        if sl is not None:
+            raise ValueError("muon updates whole matrices, not slices of the flat buffer")
+        if not prepared:
+            self.prepare_step()
+        master, low, grads = self._views()
+        at = 0
+        for g in self.groups:
+            count = len(g.offsets)
+            buf = self.buffer[at:at + count * g.size].view(count, g.m, g.n)
+            at += count * g.size
+            u = raw.muon_momentum(grads, g, buf, self.momentum, self.nesterov, self.grad_scale, self.hyper)
+            o = raw.newton_schulz(u, self.ns_steps)
+            raw.muon_apply(master, low, g, o, self.lr, max(1.0, g.m / g.n) ** 0.5, self.weight_decay, self.hyper)
+        raw.adam_pieces(master, low, grads, self.m, self.v, self.pieces, self.lr, self.beta1, self.beta2, self.eps, self.adam_weight_decay,
+                        self.step_count, self.grad_scale, self.ratio, self.hyper)
+
+    def state_dict(self):
+        d = super().state_dict()
+        d.update(lr=torch.tensor(self.lr, dtype=torch.float64), momentum=self.buffer, m=self.m, v=self.v)
+        return d
+
+    def load_state_dict(self, d):
+        super().load_state_dict(d)
+        self.buffer.copy_(d["momentum"])
+        self.m.copy_(d["m"])
+        self.v.copy_(d["v"])
+
+
 def plan_buckets(points: Sequence[int], lo: int, hi: int, n_buckets: int, min_bucket: int) -> List[tuple]:
     """Cut ``[lo, hi)`` into buckets ``(lo_i, hi_i)`` in the order backward finishes them (highest offsets first).
     ``points`` are the offsets ``Graph.grad_hook`` reports, in firing order; a bucket ends at such a point and holds
@@ -234,6 +325,8 @@ class OverlappedUpdate:
         """Needs a CUDA graph whose gradients become final in buffer order, and no entries that a decaying update
         must skip (the sliced update does not put batch-norm running statistics back)."""
         if graph.master_flat is None or graph.master_flat.device.type != "cuda" or not graph.grad_hook_usable():
+            return False
+        if isinstance(opt, Muon):  # its matrices are not updated in slices
             return False
         if getattr(opt, "weight_decay", 0.0) != 0.0 and getattr(opt, "_frozen_idx", None) is not None:
             return False
@@ -301,6 +394,10 @@ def create_optimizer(cfg: Optional[dict]) -> Optimizer:
     lr = float(cfg.get("learning_rate", cfg.get("lr", 1e-3)))
     if t == "sgd":
         return SGD(lr, float(cfg.get("momentum", 0.0)))
+    if t == "muon":
+        lr = float(cfg.get("learning_rate", cfg.get("lr", 0.02)))
+        return Muon(lr, **{k: cfg[k] for k in ("momentum", "nesterov", "ns_steps", "weight_decay", "adam_learning_rate", "beta1", "beta2",
+                                               "epsilon", "adam_weight_decay") if k in cfg})
     kw = dict(beta1=float(cfg.get("beta1", 0.9)), beta2=float(cfg.get("beta2", 0.999)), epsilon=float(cfg.get("epsilon", 1e-8)),
               weight_decay=float(cfg.get("weight_decay", 0.0)))
     if t == "adamw":

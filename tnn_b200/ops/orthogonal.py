@@ -126,3 +126,114 @@ def _address(array) -> int:
     import ctypes
 
     return ctypes.addressof(array)
+
+
+# ------------------------------------------------------------------------- the optimizer's element-wise passes
+_MUON_DECLARED = False
+
+
+def _muon_library():
+    global _MUON_DECLARED
+    lib = _lib.load()
+    if not _MUON_DECLARED:
+        p, i, l, f = _lib.c_void_p, _lib.c_int, _lib.c_ll, _lib.c_float
+        _lib.declare(lib, "tnnb_muon_momentum", [p, p, p, p, i, l, f, i, f, p, i, p])
+        _lib.declare(lib, "tnnb_muon_apply", [p, p, p, p, i, l, f, f, f, p, i, p])
+        _lib.declare(lib, "tnnb_adam_pieces", [p, p, p, p, p, p, i, f, f, f, f, f, f, f, f, f, p, p])
+        _MUON_DECLARED = True
+    return lib
+
+
+class MatrixGroup:
+    """Equal matrices inside the flat buffers of a graph: ``offsets`` (elements) of ``[m, n]`` matrices. ``device``: where the buffers
+    lie."""
+
+    def __init__(self, m: int, n: int, offsets: Sequence[int], device):
+        self.m, self.n, self.offsets = int(m), int(n), [int(o) for o in offsets]
+        if self.m <= 0 or self.n <= 0 or not self.offsets:
+            raise ValueError(f"{len(self.offsets)} matrices of {m} x {n}")
+        self.size = self.m * self.n
+        self.wide = int(self.size % 4 == 0 and all(o % 4 == 0 for o in self.offsets))
+        self.table = torch.tensor(self.offsets, dtype=torch.int64, device=device)
+
+    def check(self, flat: torch.Tensor, what: str) -> None:
+        if flat.dim() != 1 or not flat.is_contiguous() or min(self.offsets) < 0 or max(self.offsets) + self.size > flat.numel():
+            raise ValueError(f"matrices of {self.m} x {self.n} do not lie in {what} of {tuple(flat.shape)}")
+
+
+def muon_momentum(grads: torch.Tensor, group: MatrixGroup, buffer: torch.Tensor, momentum: float, nesterov: bool = True,
+                  gscale: float = 1.0, hyper=None) -> torch.Tensor:
+    """``buffer <- momentum * buffer + (1 - momentum) * g`` for the group's matrices of the flat fp32 ``grads``; returns the
+    update ``[count, m, n]`` (fp32): the buffer, or with ``nesterov`` once more mixed with the gradient."""
+    count = len(group.offsets)
+    group.check(grads, "the gradients")
+    if tuple(buffer.shape) != (count, group.m, group.n) or buffer.dtype != torch.float32 or grads.dtype != torch.float32 \
+            or not buffer.is_contiguous() or buffer.device != grads.device:
+        raise ValueError(f"momentum buffer {tuple(buffer.shape)} of {buffer.dtype} for {count} matrices of {group.m} x {group.n}")
+    if grads.is_cuda:
+        with _lib.device_of(grads):
+            u = torch.empty_like(buffer)
+            for i in range(0, count, 65535):
+                k = min(65535, count - i)
+                rc = _muon_library().tnnb_muon_momentum(grads, group.table[i:], buffer[i:], u[i:], k, group.size, momentum, int(nesterov), gscale,
+                                                        hyper, group.wide, _lib.raw_stream())
+                _lib.check_rc(rc, "muon_momentum")
+                LAUNCHES["count"] += 1
+        return u
+    g = torch.stack([grads[o:o + group.size] for o in group.offsets]).view_as(buffer) * (gscale if hyper is None else hyper[3])
+    buffer.mul_(momentum).add_(g * (1 - momentum))
+    return buffer * momentum + g * (1 - momentum) if nesterov else buffer.clone()
+
+
+def muon_apply(master: torch.Tensor, low, group: MatrixGroup, update: torch.Tensor, lr: float, factor: float, decay: float = 0.0,
+               hyper=None) -> None:
+    """``w <- w - lr * (factor * update + decay * w)`` for the group's matrices of the flat fp32 ``master``, and their rounded values into
+    ``low`` (bf16, or None)."""
+    count = len(group.offsets)
+    group.check(master, "the weights")
+    if update.numel() != count * group.size or update.dtype != torch.bfloat16 or not update.is_contiguous() \
+            or master.dtype != torch.float32 or update.device != master.device:
+        raise ValueError(f"update {tuple(update.shape)} of {update.dtype} for {count} matrices of {group.m} x {group.n}")
+    if low is not None and (low.shape != master.shape or low.dtype != torch.bfloat16 or low.device != master.device):
+        raise ValueError(f"compute copy {tuple(low.shape)} of {low.dtype} beside weights {tuple(master.shape)}")
+    update = update.view(count, -1)
+    if master.is_cuda:
+        with _lib.device_of(master):
+            for i in range(0, count, 65535):
+                k = min(65535, count - i)
+                rc = _muon_library().tnnb_muon_apply(master, low, group.table[i:], update[i:], k, group.size, lr, factor, decay, hyper, group.wide,
+                                                     _lib.raw_stream())
+                _lib.check_rc(rc, "muon_apply")
+                LAUNCHES["count"] += 1
+        return
+    rate = lr if hyper is None else hyper[0]
+    for o, u in zip(group.offsets, update):
+        w = master[o:o + group.size]
+        w.sub_(rate * (factor * u.float() + decay * w))
+        if low is not None:
+            low[o:o + group.size].copy_(w)
+
+
+def adam_pieces(master: torch.Tensor, low, grads: torch.Tensor, m: torch.Tensor, v: torch.Tensor, pieces: torch.Tensor, lr: float, b1: float,
+                b2: float, eps: float, wd: float, step: int, gscale: float = 1.0, lr_ratio: float = 1.0, hyper=None) -> None:
+    """:func:`raw.adam_step` over pieces of the flat buffers: ``pieces`` int64 ``[count, 3]``, on the buffers' device: offset, length and
+    place in the packed moments ``m``, ``v``."""
+    bc1, bc2 = 1 - b1 ** step, 1 - b2 ** step
+    if master.is_cuda:
+        with _lib.device_of(master):
+            rc = _muon_library().tnnb_adam_pieces(master, low, grads, m, v, pieces, pieces.shape[0], lr, b1, b2, eps, wd, bc1, bc2, gscale, lr_ratio,
+                                                  hyper, _lib.raw_stream())
+            _lib.check_rc(rc, "adam_pieces")
+            LAUNCHES["count"] += 1
+        return
+    if hyper is not None:
+        lr, bc1, bc2, gscale = (float(x) for x in hyper)
+    rate = lr * lr_ratio
+    for at, n, st in pieces.tolist():
+        g = grads[at:at + n].float() * gscale
+        mi, vi, w = m[st:st + n], v[st:st + n], master[at:at + n]
+        mi.mul_(b1).add_(g, alpha=1 - b1)
+        vi.mul_(b2).addcmul_(g, g, value=1 - b2)
+        w.sub_(rate * (mi / bc1) / (torch.sqrt(vi / bc2) + eps) + wd * rate * w)
+        if low is not None:
+            low[at:at + n].copy_(w.to(low.dtype))

@@ -818,5 +818,5 @@ def pool2d_bwd(dy, idx, x_shape, mode: str, pool, stride, pad):
 # The CUDA sides of the functions above; imported last because they import this package's other modules.
 from . import conv, norm  # noqa: E402
 from . import pool as pool_ops  # noqa: E402
-from .orthogonal import newton_schulz  # noqa: E402,F401
+from .orthogonal import MatrixGroup, adam_pieces, muon_apply, muon_momentum, newton_schulz  # noqa: E402,F401
 from .vocab import TokenLogProbs, embedding_grad, embedding_lookup, token_log_probs, token_log_probs_grad  # noqa: E402,F401

@@ -55,6 +55,9 @@ class FusedDPOptimizer:
 
     def __init__(self, opt: Optimizer, graph, heap: SymmetricHeap, regions: Sequence[Region], grad_scale: float,
                  overlap: bool = False, n_buckets: int = 4):
+        if opt.TYPE == "muon":
+            raise ValueError("the sharded data-parallel update works on slices of the parameters; muon needs whole matrices: "
+                             "run it with fused_collectives off")
         self.opt, self.graph, self.heap, self.regions = opt, graph, heap, list(regions)
         self.lib = _lib.load()
         _declare(self.lib)
