@@ -236,10 +236,12 @@ embed_sum_kernel(const TI* dy, long long ld, const int* order, const uint32_t* k
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const long long all = (long long)fills * gridDim.y * warps;
     const long long me = ((long long)blockIdx.y * fills + blockIdx.x) * warps + (threadIdx.x >> 5);
-    for (long long r0 = me * 32; r0 < vocab; r0 += all * 32) {
+    constexpr int SPAN = 8;  // rows a warp looks at together: few, or a small table keeps a part of the warps busy only
+    for (long long r0 = me * SPAN; r0 < vocab; r0 += all * SPAN) {
       const long long r = r0 + lane;
-      const int at = r < vocab ? slot_of(slots, (int)r) : 0;
-      unsigned empty = __ballot_sync(0xffffffffu, r < vocab && rowptr[at] == rowptr[at + 1]);
+      const bool mine = lane < SPAN && r < vocab;
+      const int at = mine ? slot_of(slots, (int)r) : 0;
+      unsigned empty = __ballot_sync(0xffffffffu, mine && rowptr[at] == rowptr[at + 1]);
       for (; empty; empty &= empty - 1)
         clear_row(reinterpret_cast<uint8_t*>(out + (r0 + __ffs(empty) - 1) * width), (long long)width * sizeof(TO), lane);
     }

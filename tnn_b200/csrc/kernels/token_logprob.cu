@@ -537,10 +537,12 @@ token_logprob_kernel(const LogprobParams a, int parts) {
   const bool nothing = tid >= r.p.v_hi - r.p.v_lo && single < 0;
   const uint32_t own_key = nothing ? 0u : key_of(top);
   if (k > 0) {
+    // groups of 4 threads; of 2 or 1 where there are no more vectors than that makes groups
+    const int share = r.p.v_hi - r.p.v_lo > 2 * LP_GROUPS ? 4 : r.p.v_hi - r.p.v_lo > LP_GROUPS ? 2 : 1;
     uint32_t g = own_key;
-#pragma unroll
-    for (int o = 1; o < LP_THREADS / LP_GROUPS; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if (tid % (LP_THREADS / LP_GROUPS) == 0) sh.group[tid / (LP_THREADS / LP_GROUPS)] = g;
+    if (share > 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, 1));
+    if (share > 2) g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+    if (tid % share == 0 && tid / share < LP_GROUPS) sh.group[tid / share] = g;
     if (tid < LP_TOP) sh.best[tid] = 0;
     if (tid == 0) sh.winners = sh.found = 0;
   }

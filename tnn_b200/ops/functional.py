@@ -181,6 +181,15 @@ def cross_entropy(logits: torch.Tensor, labels: torch.Tensor, return_corrects: b
     return (loss, corrects) if return_corrects else loss
 
 
+def _differentiable_once(backward):
+    """``once_differentiable`` where a second derivative may be asked for (``create_graph``): it costs 20 us a call."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx):
@@ -189,7 +198,7 @@ class _Embedding(torch.autograd.Function):
         return raw.embedding_lookup(ids, table, scale, padding_idx)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         rows, scale, padding_idx = ctx.args
@@ -216,7 +225,7 @@ class _TokenLogProbs(torch.autograd.Function):
         return tuple(r)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, g, h, *_):
         logits, tokens, stats, entropy = ctx.saved_tensors
         if g is None and h is None:
