@@ -208,3 +208,43 @@ def test_operators_together(dev, dtype):
         assert float((a - b).norm() / b.norm()) < tol
     own = got[3].to(torch.float32)
     assert float((got[5] - exact(own)).norm() / exact(own).norm()) < BOUND
+
+
+def test_stages_of_a_pipeline_take_the_same_matrices():
+    """The layer in front of a cut is not the model's last: all stages together orthogonalise what the whole model does."""
+    from tnn_b200.nn.graph import partition_graph
+
+    make = lambda: zoo.gpt2(64, 2, 2, "t", seq_len=16, vocab=50)  # noqa: E731
+    count = lambda opt: {(x.m, x.n): len(x.offsets) for x in opt.groups}  # noqa: E731
+    whole = count(Muon().attach(make().compile(device="cpu", seed=0)))
+    for cuts in ([1.0, 1.0], [1.0, 1.0, 1.0, 1.0, 1.0]):
+        parts = {}
+        for stage in partition_graph(make(), cuts):
+            for k, v in count(Muon().attach(stage.compile(device="cpu", seed=0))).items():
+                parts[k] = parts.get(k, 0) + v
+        assert parts == whole
+
+
+def test_refusals_of_places():
+    flat = torch.zeros(64)
+    for offsets in ([0, 0], [0, 23], [30, 8]):
+        with pytest.raises(ValueError, match="overlap"):
+            raw.MatrixGroup(4, 6, offsets, "cpu")
+    pieces = torch.tensor([[0, 8, 0]])
+    m, v = torch.zeros(8), torch.zeros(8)
+    bad = [dict(pieces=pieces.int()), dict(pieces=pieces[0]), dict(m=m.double()), dict(v=torch.zeros(9)), dict(grads=torch.zeros(63)),
+           dict(low=torch.zeros(63)), dict(master=flat.bfloat16())]
+    for change in bad:
+        args = dict(master=flat, low=None, grads=torch.zeros(64), m=m, v=v, pieces=pieces)
+        args.update(change)
+        with pytest.raises(ValueError):
+            raw.adam_pieces(*args.values(), 0.1, 0.9, 0.95, 1e-8, 0.0, 1)
+
+
+@gpu
+def test_places_on_another_device_are_refused():
+    group = raw.MatrixGroup(4, 6, [0], "cpu")
+    with pytest.raises(ValueError):
+        raw.muon_momentum(torch.zeros(24, device="cuda"), group, torch.zeros(1, 4, 6, device="cuda"), 0.9)
+    with pytest.raises(ValueError):
+        raw.muon_apply(torch.zeros(24, device="cuda"), None, group, torch.zeros(1, 4, 6, device="cuda", dtype=torch.bfloat16), 0.1, 1.0)

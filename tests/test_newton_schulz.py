@@ -169,3 +169,19 @@ def test_captured_and_replayed():
         g.copy_(matrices(3, 150, 200, "gauss", seed))
         graph.replay()
         assert torch.equal(out, raw.newton_schulz(g))
+
+
+@gpu
+def test_two_streams_at_once():
+    """Two calls in flight on two streams: each kernel's blocks run together or not yet, and neither sees the other's matrices."""
+    g = [matrices(3, 150, 200, "gradient", s).cuda() for s in (1, 2)]
+    alone = [raw.newton_schulz(x) for x in g]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(raw.newton_schulz(g[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(x, alone[i]) for x in got[i])

@@ -65,3 +65,10 @@ def test_command(capsys, tmp_path):
     summary = json.loads(lines[-1])
     assert len(lines) == 11 and summary["tokens"] == 10
     assert abs(summary["perplexity"] - math.exp(-summary["mean_log_prob"])) < 1e-6 * summary["perplexity"]
+
+
+def test_tokens_outside_the_vocabulary_are_refused():
+    g = zoo.gpt2(64, 1, 1, "t", seq_len=8, vocab=20).compile(device="cpu", seed=0)
+    for tokens in ([3, -1, 2], [3, -100, 2], [20, 1], [1, 2, 20]):
+        with pytest.raises(ValueError):
+            score_tokens(g, tokens)

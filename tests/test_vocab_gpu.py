@@ -255,3 +255,65 @@ def test_empty_batches():
     assert torch.equal(raw.embedding_grad(none, torch.zeros(2, 0, 4, device="cuda"), 3).cpu(), torch.zeros(3, 4))
     r = raw.token_log_probs(torch.zeros(2, 0, 5, device="cuda"), none, 2)
     assert r.log_probs.shape == (2, 0) and r.top_indices.shape == (2, 0, 2)
+
+
+def test_many_dimensions():
+    ids = torch.arange(6, device="cuda").view(1, 1, 2, 1, 3, 1, 1, 1, 1)
+    table = torch.randn(6, 5, device="cuda")
+    assert torch.equal(raw.embedding_lookup(ids, table), table.view(1, 1, 2, 1, 3, 1, 1, 1, 1, 5))
+    assert torch.equal(raw.embedding_grad(ids, table.view(*ids.shape, 5), 6), table)
+    z = torch.randn(6, 9, device="cuda")
+    keep, flat = {}, {}
+    r, s = raw.token_log_probs(z.view(*ids.shape, 9), ids, 2, keep=keep), raw.token_log_probs(z, ids.view(6), 2, keep=flat)
+    for a, b in zip(r, s):
+        assert torch.equal(a.reshape(b.shape), b) and a.shape[:9] == ids.shape
+    g = torch.randn(6, device="cuda")
+    assert torch.equal(raw.token_log_probs_grad(z.view(*ids.shape, 9), ids, keep, g, g).view(6, 9),
+                       raw.token_log_probs_grad(z, ids.view(6), flat, g, g))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1000, 1003])
+def test_gradient_of_the_last_positions(dtype, vocab):
+    """Rows a whole sequence apart: the gradient leaves no such gaps."""
+    z = torch.randn(5, 7, vocab).to(dtype)
+    tokens, g, h = torch.randint(0, vocab, (5,)), torch.randn(5), torch.randn(5)
+    keep = {}
+    last = z.cuda()[:, -1]
+    raw.token_log_probs(last, tokens.cuda(), keep=keep)
+    d = raw.token_log_probs_grad(last, tokens.cuda(), keep, g.cuda(), h.cuda())
+    assert d.untyped_storage().nbytes() <= 5 * (vocab + 8) * z.element_size()
+    ref, mag = logprobs_grad64(z[:, -1], tokens, g, h, 1.0, -100)
+    within(d, ref, HALF[dtype] * ref.abs() + 2.0 ** -24 * 200 * mag + TINY[dtype])
+
+
+def test_kept_statistics_of_other_rows_are_refused():
+    z, tokens, g = torch.randn(4, 30, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda"), torch.ones(4, device="cuda")
+    keep = {}
+    raw.token_log_probs(z[:3], tokens[:3], keep=keep)
+    for bad in (keep, {"stats": None, "entropy": g}, {"stats": torch.zeros(4, 2), "entropy": g}, {"stats": torch.zeros(4, 2, device="cuda"), "entropy": g.double()}):
+        with pytest.raises(ValueError):
+            raw.token_log_probs_grad(z, tokens, bad, g, None)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams side by side, each of which has workspaces of its own, give what each gives alone."""
+    ids = [ids_for(3000, 500, "zipf", s).cuda() for s in (1, 2)]
+    dy = torch.randn(3000, 136, device="cuda", dtype=torch.bfloat16)
+    z = [torch.randn(40, 20001, device="cuda") for _ in range(2)]
+    tokens = torch.arange(40, device="cuda")
+
+    def work(i):
+        return [raw.embedding_grad(ids[i], dy, 500), *raw.token_log_probs(z[i], tokens, 8)]
+
+    alone = [work(0), work(1)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, alone[i]))

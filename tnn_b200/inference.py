@@ -98,6 +98,8 @@ def score_tokens(graph: Graph, tokens: Iterable[int], top_k: int = 0, temperatur
     n = ids.numel()
     if n < 2:
         raise ValueError(f"a text of {n} tokens has none behind its first")
+    if int(ids.min()) < 0:
+        raise ValueError(f"token {int(ids.min())}")
     S = seq_len or model_seq_len(graph) or n
     context = S // 2 if context is None else int(context)
     if not 0 <= context < S or batch < 1:
@@ -120,6 +122,8 @@ def score_tokens(graph: Graph, tokens: Iterable[int], top_k: int = 0, temperatur
                 known = min(S, n - 1 - s)
                 y[r, skip:known] = ids[s + 1 + skip:s + 1 + known]
             logits = graph.forward({graph.input_nodes[0].uid(): x.to(graph.device)})[graph.output_nodes[0].uid()]
+            if int(ids.max()) >= logits.shape[-1]:
+                raise ValueError(f"token {int(ids.max())} of a vocabulary of {logits.shape[-1]}")
             r = raw.token_log_probs(logits, y.to(graph.device), top_k, temperature)
             keep = (y != -100).reshape(-1).nonzero()[:, 0].to(graph.device)
             parts.append([t.flatten(0, 1).index_select(0, keep) for t in r])

@@ -164,6 +164,7 @@ class Graph:
         self.segments: List["_Segment"] = []
         self.fuse = True
         self.batch_independent = True
+        self.ends_model = True  # False for a pipeline stage with others behind it
 
     # ------------------------------------------------------------------ construction
     def _gen_uid(self) -> str:
@@ -734,6 +735,7 @@ def partition_graph(graph: "Graph", ratios: Sequence[float]) -> List["Graph"]:
             g.add_edge(graph.edges[eid].layer, [nodes[i] for i in prod], [nodes[i] for i in cons])
         g.start_layer, g.layer_count = int(p["start_layer"]), int(p["layer_count"])
         g.input_uids, g.output_uids = list(p["input_uids"]), list(p["output_uids"])
+        g.ends_model = p is parts[-1]
         stages.append(g)
     return stages
 

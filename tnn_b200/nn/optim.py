@@ -195,7 +195,7 @@ class Muon(Optimizer):
     Every dense, attention and convolution weight is a matrix ``[outputs, inputs]`` (a filter ``[O, KH, KW, I]`` as
     ``[O, KH * KW * I]``): ``buffer = mu * buffer + (1 - mu) * g``, Nesterov's mix of buffer and gradient, five Newton-Schulz steps
     (:func:`raw.newton_schulz`, all equal matrices of the model at once), ``w -= lr * (scale * update + weight_decay * w)`` with
-    ``scale = max(1, outputs / inputs) ** 0.5``. Embeddings, the layer that makes the graph's output, norms and biases take AdamW
+    ``scale = max(1, outputs / inputs) ** 0.5``. Embeddings, the layer that makes the model's output, norms and biases take AdamW
     with ``adam_learning_rate`` (schedulers move both rates in proportion). The reference has no such optimizer."""
     TYPE = "muon"
     PIECE = 4096  # elements of the other parameters per block of the AdamW launch
@@ -221,7 +221,7 @@ class Muon(Optimizer):
         self.graph = graph
         dev = graph.master_flat.device
         outputs = {id(n) for n in graph.output_nodes}
-        last = {id(e.layer) for e in graph.edges if any(id(c) in outputs for c in e.consumers)}
+        last = {id(e.layer) for e in graph.edges if graph.ends_model and any(id(c) in outputs for c in e.consumers)}
         shapes: Dict[tuple, List[int]] = {}
         rest = []
         for layer in graph.layers():

@@ -153,10 +153,15 @@ class MatrixGroup:
         if self.m <= 0 or self.n <= 0 or not self.offsets:
             raise ValueError(f"{len(self.offsets)} matrices of {m} x {n}")
         self.size = self.m * self.n
+        order = sorted(self.offsets)
+        if any(b - a < self.size for a, b in zip(order, order[1:])):
+            raise ValueError(f"matrices of {m} x {n} at {order} overlap")
         self.wide = int(self.size % 4 == 0 and all(o % 4 == 0 for o in self.offsets))
         self.table = torch.tensor(self.offsets, dtype=torch.int64, device=device)
 
     def check(self, flat: torch.Tensor, what: str) -> None:
+        if flat.device != self.table.device:
+            raise ValueError(f"{what} on {flat.device}, the matrices' places on {self.table.device}")
         if flat.dim() != 1 or not flat.is_contiguous() or min(self.offsets) < 0 or max(self.offsets) + self.size > flat.numel():
             raise ValueError(f"matrices of {self.m} x {self.n} do not lie in {what} of {tuple(flat.shape)}")
 
@@ -196,6 +201,8 @@ def muon_apply(master: torch.Tensor, low, group: MatrixGroup, update: torch.Tens
         raise ValueError(f"update {tuple(update.shape)} of {update.dtype} for {count} matrices of {group.m} x {group.n}")
     if low is not None and (low.shape != master.shape or low.dtype != torch.bfloat16 or low.device != master.device):
         raise ValueError(f"compute copy {tuple(low.shape)} of {low.dtype} beside weights {tuple(master.shape)}")
+    if low is not None and not low.is_contiguous():
+        raise ValueError("a compute copy with gaps")
     update = update.view(count, -1)
     if master.is_cuda:
         with _lib.device_of(master):
@@ -217,7 +224,15 @@ def muon_apply(master: torch.Tensor, low, group: MatrixGroup, update: torch.Tens
 def adam_pieces(master: torch.Tensor, low, grads: torch.Tensor, m: torch.Tensor, v: torch.Tensor, pieces: torch.Tensor, lr: float, b1: float,
                 b2: float, eps: float, wd: float, step: int, gscale: float = 1.0, lr_ratio: float = 1.0, hyper=None) -> None:
     """:func:`raw.adam_step` over pieces of the flat buffers: ``pieces`` int64 ``[count, 3]``, on the buffers' device: offset, length and
-    place in the packed moments ``m``, ``v``."""
+    place in the packed moments ``m``, ``v``; no element in two pieces."""
+    for t, what in ((master, "weights"), (grads, "gradients"), (m, "moments"), (v, "moments")):
+        if t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous() or t.device != master.device:
+            raise ValueError(f"{what} {tuple(t.shape)} of {t.dtype} on {t.device}: packed fp32 on {master.device} expected")
+    if pieces.dim() != 2 or pieces.shape[1] != 3 or pieces.dtype != torch.int64 or pieces.device != master.device or not pieces.is_contiguous():
+        raise ValueError(f"pieces {tuple(pieces.shape)} of {pieces.dtype} on {pieces.device}: int64 [count, 3] on {master.device} expected")
+    if grads.shape != master.shape or m.shape != v.shape or (low is not None and (low.shape != master.shape or low.device != master.device)) \
+            or (low is not None and master.is_cuda and (low.dtype != torch.bfloat16 or not low.is_contiguous())):
+        raise ValueError("weights, gradients and compute copy, or the moments, differ in shape, or the copy is not packed bf16")
     bc1, bc2 = 1 - b1 ** step, 1 - b2 ** step
     if master.is_cuda:
         with _lib.device_of(master):

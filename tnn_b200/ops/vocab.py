@@ -65,6 +65,10 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     return t if (t.stride(1) == 1 or width == 1) and (t.shape[0] < 2 or t.stride(0) >= width) else t.contiguous()
 
 
+def _new(like: torch.Tensor, dtype, *sizes: int) -> torch.Tensor:
+    return _lib.empty(like, dtype, *sizes) if len(sizes) <= 8 else torch.empty(sizes, dtype=dtype, device=like.device)
+
+
 def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]  # the stride of a single row means nothing
 
@@ -85,7 +89,7 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         code = _type_code(table, "embedding table")
         table = _rows(table, width)
         with _lib.device_of(table):
-            out = _lib.empty(table, *ids.shape, width)
+            out = _new(table, table.dtype, *ids.shape, width)
             if n:
                 rc = _library().tnnb_embed_lookup(flat, flat.dtype is torch.int64, table.data_ptr(), max(_pitch(table), width), out, n, width, rows, pad,
                                                   float(scale), code, _lib.raw_stream())
@@ -200,8 +204,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
         code = _type_code(logits, "logits")
         with _lib.device_of(z):
             f32 = torch.float32
-            lp, ent = _lib.empty(z, f32, *shape), _lib.empty(z, f32, *shape)
-            top, idx = _lib.empty(z, f32, *shape, top_k), _lib.empty(z, torch.int64, *shape, top_k)
+            lp, ent = _new(z, f32, *shape), _new(z, f32, *shape)
+            top, idx = _new(z, f32, *shape, top_k), _new(z, torch.int64, *shape, top_k)
             stats = _lib.empty(z, f32, rows, 2) if keep is not None else None
             if rows:
                 rc = _library().tnnb_token_logprob(z.data_ptr(), max(_pitch(z), V), tok, tok.dtype is torch.int64, lp, ent, top, idx, stats, rows, V, top_k,
@@ -245,8 +249,8 @@ def _distribution(z: torch.Tensor, temperature: float) -> Tuple[torch.Tensor, to
 def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict, g_log_probs: Optional[torch.Tensor],
                          g_entropy: Optional[torch.Tensor], temperature: float = 1.0, ignore_index: int = -100) -> torch.Tensor:
     """Gradient with respect to ``logits`` for gradients of the log probabilities and the entropies (None: zero). ``kept``: what the
-    forward call left in its ``keep``. Rows without a distribution get zeros. The result has the shape of ``logits`` and, where their
-    rows lie apart, the same distance between rows."""
+    forward call left in its ``keep``. Rows without a distribution get zeros. The result has the shape of ``logits`` and, where the
+    gaps between its rows are smaller than a row, the same gaps."""
     V = _check_rows(logits, tokens, 0, float(temperature))
     tok = _whole(tokens, logits, "tokens")
     z = _rows(logits, V)
@@ -262,18 +266,25 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
     g, h = grad_of(g_log_probs), grad_of(g_entropy)
     if logits.is_cuda:
         code = _type_code(logits, "logits")
+        stats, entropy = kept["stats"], kept["entropy"]
+        for t, size, what in ((stats, 2 * rows, "statistics"), (entropy, rows, "entropies")):
+            if t is None or t.dtype is not torch.float32 or t.numel() != size or t.device != z.device or not t.is_contiguous():
+                raise ValueError(f"the {what} that were kept do not belong to {rows} rows on {z.device}")
         with _lib.device_of(z):
             pitch = max(_pitch(z), V)
-            dz = _lib.empty(z, rows, pitch)
-            if pitch != V:
+            # rows far apart (the last position of every sequence): not that much memory between those of the result, and the same
+            # place within 16 bytes, so that rows of both share vectors
+            out_pitch = pitch if pitch < 2 * V else V + (pitch - V) % 8
+            dz = _lib.empty(z, rows, out_pitch)
+            if out_pitch != V:
                 dz = dz[:, :V]
             if rows:
-                rc = _library().tnnb_token_logprob_grad(z.data_ptr(), pitch, dz, pitch, tok, tok.dtype is torch.int64, kept["stats"], kept["entropy"],
+                rc = _library().tnnb_token_logprob_grad(z.data_ptr(), pitch, dz, out_pitch, tok, tok.dtype is torch.int64, stats, entropy,
                                                         g, h, rows, V, _LOG2E / float(temperature), 1.0 / float(temperature),
                                                         int(ignore_index), code, _lib.raw_stream())
                 _lib.check_rc(rc, "token_log_probs_grad")
                 LAUNCHES["count"] += 1
-        return dz.view(logits.shape) if pitch == V else dz.unflatten(0, logits.shape[:-1])
+        return dz.view(logits.shape) if out_pitch == V else dz.unflatten(0, logits.shape[:-1])
     tok = tok.reshape(-1)
     zf = z.to(torch.promote_types(z.dtype, torch.float32))
     logp, p, plogp = _distribution(zf, float(temperature))

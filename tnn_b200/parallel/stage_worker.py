@@ -101,6 +101,7 @@ class StageWorker:
         st = msg["stage"]
         self.graph = Graph.from_state(tnng.parse(bytes(st["graph_state"])), device=self.device)
         self.graph.input_requires_grad = bool(st["prev_stage"])
+        self.graph.ends_model = not st["next_stage"]
         self.optimizer = create_optimizer(json.loads(st["optimizer_config"] or "{}")).attach(self.graph)
         self.scheduler = create_scheduler(json.loads(st["scheduler_config"] or "{}"), self.optimizer)
         self.next_stage, self.prev_stage = st["next_stage"], st["prev_stage"]
