@@ -56,14 +56,17 @@ embed_lookup_kernel(const ID* __restrict__ ids, const T* __restrict__ table, lon
 // Positions sorted by token, in an order that depends on the ids alone, without a pass over global counters: every CTA owns some table rows, reads ALL ids (they come
 // from L2: 64 KB for 8192 tokens) and picks its own. The number of ids that belong to CTAs before it is the place of its part of
 // the list, so no CTA waits for another. Within the CTA each warp walks a contiguous stretch of the ids and has a counter per row:
-// counts, then starting places (rows ascending, warps ascending within a row), then the places themselves. A place gets its token with
+// counts, then starting places (rows ascending, warps ascending within a row), then the places themselves. On the first look it notes the
+// positions that are its CTA's, as many as there is room for; a warp with more of them (a token that fills the batch) looks at its
+// stretch again. A place gets its token with
 // two flags, so that what adds up needs no other table: whether it is the token's first position and whether it is its last.
 //
 // Rows are dealt out in turn (2^bits CTAs; row v is number v >> bits of CTA v mod 2^bits): frequent tokens have neighbouring numbers, and
 // with ranges of rows the CTA that had them took 16 us for 8192 tokens of text, 63 for 50001. The list is in this order of rows
-// ("slots"), which is as good as any.
+// ("slots"), which is as good as any. Looking twice at every position cost 10 us of 97 for 50001 positions of 1001 fp32 columns.
 static constexpr int SORT_WARPS = 32;
 static constexpr int SORT_ROWS = 512;  // most rows of a CTA, one per thread
+static constexpr int SORT_NOTES = 128;  // positions that a warp notes: row in 9 bits, place in its stretch in 23
 static constexpr uint32_t TOKEN_FIRST = 1u << 30, TOKEN_LAST = 1u << 31, TOKEN_ROW = TOKEN_FIRST - 1;
 
 struct Slots {
@@ -100,6 +103,7 @@ embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_
   extern __shared__ int counters[];  // [SORT_WARPS][slots.rows]
   __shared__ int below[SORT_WARPS], scan[SORT_WARPS];
   __shared__ int begin[SORT_ROWS], count[SORT_ROWS];
+  __shared__ uint32_t notes[SORT_WARPS][SORT_NOTES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = slots.rows, own = blockIdx.x, mask = (1 << slots.bits) - 1;
   for (int i = threadIdx.x; i < SORT_WARPS * rows; i += blockDim.x) counters[i] = 0;
@@ -113,7 +117,7 @@ embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_
   // Calls f(four codes, place of the first) for the warp's positions, 128 at a time; the next ones are on their way meanwhile. (`codes`
   // begins on 16 bytes and ends on a whole vector.)
   auto walk = [&](auto f) {
-    constexpr int SETS = 2;
+    constexpr int SETS = 4;
     uint4 now[SETS], next[SETS];
     auto load = [&](int i0, uint4 (&v)[SETS]) {
 #pragma unroll
@@ -134,12 +138,25 @@ embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_
       }
     }
   };
-  int less = 0;
-  walk([&](const uint32_t (&w)[4], int) {
+  int less = 0, noted = stretch < 1 << 23 ? 0 : SORT_NOTES + 1;
+  walk([&](const uint32_t (&w)[4], int position) {
+    bool any = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       less += w[j] < base;
-      if (w[j] - base < 65536u) atomicAdd(&mine[w[j] & 0xffffu], 1);
+      any |= w[j] - base < 65536u;
+    }
+    if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = w[j] - base < 65536u;
+      const unsigned who = __ballot_sync(0xffffffffu, in);
+      const int at = noted + __popc(who & ((1u << lane) - 1));
+      if (in) {
+        atomicAdd(&mine[w[j] & 0xffffu], 1);
+        if (at < SORT_NOTES) notes[warp][at] = (w[j] & 0xffffu) << 23 | (uint32_t)(position + j - lo);
+      }
+      noted = min(noted + __popc(who), SORT_NOTES + 1);  // (one more: there was no room)
     }
   });
 #pragma unroll
@@ -179,30 +196,32 @@ embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_
   }
   __syncthreads();
 
-  walk([&](const uint32_t (&w)[4], int position) {
-    bool any = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) any |= w[j] - base < 65536u;
-    if (!__any_sync(0xffffffffu, any)) return;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool in = w[j] - base < 65536u;
-      const unsigned who = __ballot_sync(0xffffffffu, in);
-      if (who == 0) continue;
-      if (in) {
-        const int at = w[j] & 0xffffu;
-        // lanes with the same row, in their order
-        const unsigned same = (who & (who - 1)) ? __match_any_sync(who, at) : who;
-        const int to = mine[at] + __popc(same & ((1u << lane) - 1));
-        order[to] = position + j;
-        keys[to] = ((uint32_t)at << slots.bits | (uint32_t)own) | (to == begin[at] ? TOKEN_FIRST : 0u) |
-                   (to + 1 == begin[at] + count[at] ? TOKEN_LAST : 0u);
-        __syncwarp(same);
-        if ((same & ((1u << lane) - 1)) == 0) mine[at] = to + __popc(same);
-      }
-      __syncwarp();
+  // Lanes with `in` put position `i` of row `at` in its place, lanes of the same row in their order.
+  auto place = [&](bool in, int at, int i) {
+    const unsigned who = __ballot_sync(0xffffffffu, in);
+    if (who == 0) return;
+    if (in) {
+      const unsigned same = (who & (who - 1)) ? __match_any_sync(who, at) : who;
+      const int to = mine[at] + __popc(same & ((1u << lane) - 1));
+      order[to] = i;
+      keys[to] = ((uint32_t)at << slots.bits | (uint32_t)own) | (to == begin[at] ? TOKEN_FIRST : 0u) |
+                 (to + 1 == begin[at] + count[at] ? TOKEN_LAST : 0u);
+      __syncwarp(same);
+      if ((same & ((1u << lane) - 1)) == 0) mine[at] = to + __popc(same);
     }
-  });
+    __syncwarp();
+  };
+  if (noted <= SORT_NOTES) {
+    for (int i = lane; i - lane < noted; i += 32) {
+      const uint32_t note = i < noted ? notes[warp][i] : 0u;
+      place(i < noted, (int)(note >> 23), lo + (int)(note & 0x7fffffu));
+    }
+  } else {
+    walk([&](const uint32_t (&w)[4], int position) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) place(w[j] - base < 65536u, (int)(w[j] & 0xffffu), position + j);
+    });
+  }
 }
 
 // -------------------------------------------------------------------------------------------------------------- sums
@@ -227,7 +246,7 @@ __device__ __forceinline__ void clear_row(uint8_t* row, long long bytes, int lan
 template <typename TI, typename TO, int VEC, int COLS>
 __global__ void __launch_bounds__(256)
 embed_sum_kernel(const TI* dy, long long ld, const int* order, const uint32_t* keys, const int* rowptr, long long vocab, Slots slots,
-                 TO* out, float* parts, int width, int chunk, int fills, float scale, int accumulate) {
+                 TO* out, float* parts, int positions, int width, int chunk, int fills, float scale, int accumulate) {
   extern __shared__ int places[];  // [chunk] positions, [chunk] tokens
   grid_dep_wait();
   const int sums = gridDim.x - fills;
@@ -247,14 +266,14 @@ embed_sum_kernel(const TI* dy, long long ld, const int* order, const uint32_t* k
     }
     return;
   }
-  const int n = rowptr[slots.rows << slots.bits], me = blockIdx.x;
+  const int me = blockIdx.x;
   const long long first = (long long)me * chunk;
-  const int count = (int)min((long long)chunk, n - first);
   uint32_t* token = reinterpret_cast<uint32_t*>(places + chunk);
-  for (int i = threadIdx.x; i < count; i += blockDim.x) {
+  for (int i = threadIdx.x; i < chunk && first + i < positions; i += blockDim.x) {  // (those of padding too: their number is on its way)
     places[i] = order[first + i];
     token[i] = keys[first + i];
   }
+  const int count = (int)min((long long)chunk, rowptr[slots.rows << slots.bits] - first);
   __syncthreads();
   if (count <= 0) return;
   const int col0 = (blockIdx.y * COLS * blockDim.x + threadIdx.x) * VEC, step = blockDim.x * VEC;
@@ -317,13 +336,14 @@ static constexpr int JOIN_COLS = 128, JOIN_WARPS = 8;
 template <typename TO>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
 embed_join_kernel(const float* parts, const uint32_t* keys, const int* rowptr, Slots slots, TO* out, int width, int chunk, float scale,
-                  int accumulate) {
+                  int accumulate) {  // CTA i: the places of chunk i and one more exist
   __shared__ float sums[JOIN_WARPS][JOIN_COLS];
   grid_dep_wait();
-  const int n = rowptr[slots.rows << slots.bits];
   const long long next = ((long long)blockIdx.x + 1) * chunk;
-  if (next >= n || (keys[next - 1] & TOKEN_LAST)) return;
-  const uint32_t token = keys[next - 1] & TOKEN_ROW;
+  const int n = rowptr[slots.rows << slots.bits];
+  const uint32_t key = keys[next - 1];
+  if (next >= n || (key & TOKEN_LAST)) return;
+  const uint32_t token = key & TOKEN_ROW;
   const int at = slot_of(slots, (int)token);
   if (rowptr[at] < next - chunk) return;  // begins in an earlier chunk
   const int more = (int)((rowptr[at + 1] - 1) / chunk - blockIdx.x);  // chunks after this one
@@ -363,11 +383,11 @@ static cudaError_t sum_and_join(const void* dy, long long ld, const int* order, 
   cudaError_t e;
   if (wide) {
     auto kern = embed_sum_kernel<TI, TO, PER16, 1>;
-    e = launch_dependent(kern, grid, dim3(threads), smem, st, (const TI*)dy, ld, order, keys, rowptr, vocab, slots, (TO*)out, parts, width,
+    e = launch_dependent(kern, grid, dim3(threads), smem, st, (const TI*)dy, ld, order, keys, rowptr, vocab, slots, (TO*)out, parts, n, width,
                          chunk, fills, scale, accumulate);
   } else {
     auto kern = embed_sum_kernel<TI, TO, 1, 4>;
-    e = launch_dependent(kern, grid, dim3(threads), smem, st, (const TI*)dy, ld, order, keys, rowptr, vocab, slots, (TO*)out, parts, width,
+    e = launch_dependent(kern, grid, dim3(threads), smem, st, (const TI*)dy, ld, order, keys, rowptr, vocab, slots, (TO*)out, parts, n, width,
                          chunk, fills, scale, accumulate);
   }
   if (e != cudaSuccess || chunks == 1) return e;
