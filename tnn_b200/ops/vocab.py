@@ -174,9 +174,10 @@ class TokenLogProbs(NamedTuple):
 
 
 def _check_rows(logits, tokens, top_k, temperature):
-    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape or not logits.is_floating_point():
-        raise ValueError(f"logits {tuple(logits.shape)} of {logits.dtype} do not belong to tokens {tuple(tokens.shape)}")
-    V = logits.shape[-1]
+    shape = logits.shape
+    if not shape or shape[:-1] != tokens.shape or not logits.is_floating_point():
+        raise ValueError(f"logits {tuple(shape)} of {logits.dtype} do not belong to tokens {tuple(tokens.shape)}")
+    V = shape[-1]
     if V == 0 or V >= 1 << 30:
         raise ValueError(f"a vocabulary of {V} tokens")
     if not 0 <= top_k <= min(MAX_TOP, V):
@@ -246,6 +247,10 @@ def _distribution(z: torch.Tensor, temperature: float) -> Tuple[torch.Tensor, to
     return logp, p, plogp
 
 
+def _kept(t: Optional[torch.Tensor], size: int, z: torch.Tensor) -> bool:
+    return t is not None and t.dtype is torch.float32 and t.numel() == size and t.device == z.device and t.is_contiguous()
+
+
 def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict, g_log_probs: Optional[torch.Tensor],
                          g_entropy: Optional[torch.Tensor], temperature: float = 1.0, ignore_index: int = -100) -> torch.Tensor:
     """Gradient with respect to ``logits`` for gradients of the log probabilities and the entropies (None: zero). ``kept``: what the
@@ -261,15 +266,16 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
             return None
         if g.numel() != rows or g.device != z.device:
             raise ValueError(f"a gradient of {g.numel()} values on {g.device} for {rows} rows on {z.device}")
+        if g.dtype is torch.float32 and g.dim() == 1 and g.is_contiguous() and z.dtype is not torch.float64:
+            return g
         return g.reshape(-1).to(torch.promote_types(z.dtype, torch.float32)).contiguous()
 
     g, h = grad_of(g_log_probs), grad_of(g_entropy)
     if logits.is_cuda:
         code = _type_code(logits, "logits")
         stats, entropy = kept["stats"], kept["entropy"]
-        for t, size, what in ((stats, 2 * rows, "statistics"), (entropy, rows, "entropies")):
-            if t is None or t.dtype is not torch.float32 or t.numel() != size or t.device != z.device or not t.is_contiguous():
-                raise ValueError(f"the {what} that were kept do not belong to {rows} rows on {z.device}")
+        if not (_kept(stats, 2 * rows, z) and _kept(entropy, rows, z)):
+            raise ValueError(f"the statistics that were kept do not belong to {rows} rows on {z.device}")
         with _lib.device_of(z):
             pitch = max(_pitch(z), V)
             # rows far apart (the last position of every sequence): not that much memory between those of the result, and the same
@@ -284,6 +290,8 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
                                                         int(ignore_index), code, _lib.raw_stream())
                 _lib.check_rc(rc, "token_log_probs_grad")
                 LAUNCHES["count"] += 1
+        if logits.dim() == 2:
+            return dz
         return dz.view(logits.shape) if out_pitch == V else dz.unflatten(0, logits.shape[:-1])
     tok = tok.reshape(-1)
     zf = z.to(torch.promote_types(z.dtype, torch.float32))
