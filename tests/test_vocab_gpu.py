@@ -97,7 +97,7 @@ KINDS = ["plain", "masked", "few", "equal", "coarse", "rising", "peaked", "large
 
 
 def _tolerances(z, tokens, lp, ent, vocab, temperature):
-    """Steps of 2^-24: a thread adds up vocab / 256 / parts terms one after the other, then 8 + 8 + 8 joins; each exponent is off
+    """Steps of 2^-24: each of a thread's four sums takes up to vocab / 256 terms one after the other (64 threads or more), then 8 + 8 + 8 joins; each exponent is off
     by half a step of itself and each exponential by four (the instruction's two, and the product it is taken of); log2(e) / T is
     rounded (relative to the exponent), the result is rounded. Rounding the maximum's exponent is common to all terms and cancels."""
     chain = vocab / 256 + 24 + 8
@@ -317,3 +317,20 @@ def test_two_streams_at_once():
     for i in (0, 1):
         for r in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(r, alone[i]))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1190, 4099), (1190, 40001), (3000, 2100), (2961, 4100), (100, 5000), (150, 17000)])
+def test_rows_of_every_length_agree(rows, vocab):
+    """Few and many rows are worked on by CTAs of different sizes: the same row gives the same alternatives, and the numbers up to the order
+    of its sums."""
+    z = (torch.randn(rows, vocab, generator=torch.Generator().manual_seed(vocab)) * 3).to(torch.bfloat16)
+    z[1], z[2, : vocab // 2], z[3] = -math.inf, -math.inf, 1.0
+    z[4, 7] = z[4, vocab - 1] = 60.0
+    tokens = torch.arange(rows) % vocab
+    many = raw.token_log_probs(z.cuda(), tokens.cuda(), 9)
+    some = torch.cat([torch.arange(8), torch.arange(rows - 3, rows)])
+    lp, ent, tv, ti, *_ = logprobs64(z[some], tokens[some], 9, 1.0, -100)
+    assert torch.equal(many.top_indices.cpu()[some], ti)
+    tol_lp, tol_ent = _tolerances(z[some], tokens[some], lp, ent, vocab, 1.0)
+    within(many.log_probs[some.cuda()], lp, tol_lp)
+    within(many.entropy[some.cuda()], ent, tol_ent)

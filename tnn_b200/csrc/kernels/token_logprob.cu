@@ -8,7 +8,7 @@
 // maximum turns up; they are joined per warp, block and cluster in a fixed order. fp32 throughout, logarithms of the sums in fp64.
 //
 // The top alternatives need no second pass over the row. The k-th largest of 64 disjoint groups' maxima bounds the k-th largest logit
-// from below; only threads whose own maximum reaches that bound look at their elements again (about k of 256), and what they
+// from below; only threads whose own maximum reaches that bound look at their elements again (about k of them), and what they
 // find, a few more than k values, is ranked by counting. Order: larger logit first, then the lower index; NaN before everything, as in
 // torch's sorts. Rows with so many equal values that the candidates do not fit (all masked, all zero) find the k-th value by
 // bisection over its bits instead.
@@ -25,7 +25,6 @@ TNNB_BOUNDS_TU(token_logprob)
 
 namespace tnnb {
 
-static constexpr int LP_THREADS = 256;
 static constexpr int LP_TOP = 32;      // most alternatives
 static constexpr int LP_GROUPS = 64;   // groups of threads whose maxima bound the k-th value
 static constexpr int LP_CAND = 1024;   // candidates that fit
@@ -62,8 +61,11 @@ template <typename T> struct Logits;
 template <>
 struct Logits<float> {
   static constexpr uint32_t NONE = 0xff800000u;  // -inf
+  static constexpr float MOST = 3e38f;           // a finite value below +inf
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
   static __device__ __forceinline__ float largest(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ bool above(uint32_t w, uint32_t limit) { return !(__uint_as_float(w) <= __uint_as_float(limit)); }
+  static __device__ __forceinline__ uint32_t word(float x) { return __float_as_uint(x); }
   static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[2]) {
     x[0] = pack_f2(fmaxf(__uint_as_float(v.x), LP_LOWEST), fmaxf(__uint_as_float(v.y), LP_LOWEST));
     x[1] = pack_f2(fmaxf(__uint_as_float(v.z), LP_LOWEST), fmaxf(__uint_as_float(v.w), LP_LOWEST));
@@ -76,12 +78,23 @@ struct Logits<float> {
 template <>
 struct Logits<__nv_bfloat16> {
   static constexpr uint32_t NONE = 0xff80ff80u;
+  static constexpr float MOST = 3e38f;
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
   static __device__ __forceinline__ float largest(uint32_t w) { return max_nan(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+  // Whether one of the two elements is not below or equal to its limit; the word that holds x twice.
+  static __device__ __forceinline__ bool above(uint32_t w, uint32_t limit) {
+    uint32_t p;
+    asm("{ .reg .pred a, b; setp.gtu.bf16x2 a|b, %1, %2; or.pred a, a, b; selp.u32 %0, 1, 0, a; }" : "=r"(p) : "r"(w), "r"(limit));
+    return p != 0;
+  }
+  static __device__ __forceinline__ uint32_t word(float x) {
+    const __nv_bfloat162 h = __float2bfloat162_rn(x);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
   static __device__ __forceinline__ void pairs(const uint4& v, uint64_t (&x)[4]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -102,10 +115,20 @@ struct Logits<__nv_bfloat16> {
 template <>
 struct Logits<__half> {
   static constexpr uint32_t NONE = 0xfc00fc00u;
+  static constexpr float MOST = 65504.f;
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+  }
+  static __device__ __forceinline__ bool above(uint32_t w, uint32_t limit) {
+    uint32_t p;
+    asm("{ .reg .pred a, b; setp.gtu.f16x2 a|b, %1, %2; or.pred a, a, b; selp.u32 %0, 1, 0, a; }" : "=r"(p) : "r"(w), "r"(limit));
+    return p != 0;
+  }
+  static __device__ __forceinline__ uint32_t word(float x) {
+    const __half2 h = __float2half2_rn(x);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ void values(uint32_t w, float (&x)[2]) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -130,13 +153,13 @@ struct Logits<__half> {
     reinterpret_cast<uint32_t*>(&v)[pair] = *reinterpret_cast<const uint32_t*>(&h);
   }
 };
+// The larger elements of N vectors and a word, in the two places of a word.
 template <typename T, int N>
-__device__ __forceinline__ float vec_max(const uint4 (&v)[N]) {
+__device__ __forceinline__ uint32_t larger_of(uint32_t m, const uint4 (&v)[N]) {
   using L = Logits<T>;
-  uint32_t m = L::larger(L::larger(v[0].x, v[0].y), L::larger(v[0].z, v[0].w));
 #pragma unroll
-  for (int i = 1; i < N; ++i) m = L::larger(m, L::larger(L::larger(v[i].x, v[i].y), L::larger(v[i].z, v[i].w)));
-  return L::largest(m);
+  for (int i = 0; i < N; ++i) m = L::larger(m, L::larger(L::larger(v[i].x, v[i].y), L::larger(v[i].z, v[i].w)));
+  return m;
 }
 
 // Order of logits as unsigned integers (0: none at all), NaN above +inf, -0 equal to +0.
@@ -210,17 +233,18 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+template <int NT>  // threads of a CTA
 struct LogprobShared {
   union {
-    uint4 ring[LP_RING][LP_VECS][LP_THREADS];  // until the row has been read
+    uint4 ring[LP_RING][LP_VECS][NT];  // until the row has been read
     unsigned long long cand[LP_CAND];
   };
-  uint32_t group[LP_GROUPS];
+  alignas(16) uint32_t group[LP_GROUPS];
   uint32_t bound;
   int winners, found, total;
-  int winner[LP_THREADS];
-  int warp_count[LP_THREADS / 32];
-  Sums part[LP_THREADS / 32];
+  int winner[NT];
+  int warp_count[NT / 32];
+  Sums part[NT / 32];
   Sums all;
   unsigned long long best[LP_TOP];  // this CTA's, in order; 0 past the last
 };
@@ -264,11 +288,11 @@ __device__ __forceinline__ int loose(const RowPart& p, int i) {
 }
 
 // Number of keys >= x in the part (block-wide; every thread gets it).
-template <typename T>
-__device__ int count_from(const RowReader<T>& r, uint32_t x, LogprobShared& sh) {
+template <typename T, int NT>
+__device__ int count_from(const RowReader<T>& r, uint32_t x, LogprobShared<NT>& sh) {
   constexpr int PER = 16 / sizeof(T);
   int n = 0;
-  for (int v = r.p.v_lo + (int)threadIdx.x; v < r.p.v_hi; v += LP_THREADS) {
+  for (int v = r.p.v_lo + (int)threadIdx.x; v < r.p.v_hi; v += NT) {
     const Vec<T, PER> w = r.vec(v);
 #pragma unroll
     for (int j = 0; j < PER; ++j) n += key_of(to_f32(w.v[j])) >= x;
@@ -280,28 +304,31 @@ __device__ int count_from(const RowReader<T>& r, uint32_t x, LogprobShared& sh) 
   __syncthreads();
   n = 0;
 #pragma unroll
-  for (int w = 0; w < LP_THREADS / 32; ++w) n += sh.warp_count[w];
+  for (int w = 0; w < NT / 32; ++w) n += sh.warp_count[w];
   __syncthreads();
   return n;
 }
 
-__device__ __forceinline__ void add_candidate(LogprobShared& sh, uint32_t key, int index) {
+template <int NT>
+__device__ __forceinline__ void add_candidate(LogprobShared<NT>& sh, uint32_t key, int index) {
   const int at = atomicAdd(&sh.found, 1);
   if (at < LP_CAND) sh.cand[at] = ((unsigned long long)key << 32) | (uint32_t)~index;
 }
 
 // The elements with keys >= `from` among those of the listed threads become candidates. Returns their number (of which LP_CAND at most
-// are kept). Block-wide.
-template <typename T>
-__device__ int collect(const RowReader<T>& r, uint32_t from, LogprobShared& sh) {
+// are kept). Block-wide. None of them is below `least`, whose vectors need no closer look.
+template <typename T, int NT>
+__device__ int collect(const RowReader<T>& r, uint32_t from, float least, LogprobShared<NT>& sh) {
   constexpr int PER = 16 / sizeof(T);
-  const int each = (r.p.v_hi - r.p.v_lo + LP_THREADS - 1) / LP_THREADS + 1;  // a thread's vectors and its loose element
-  for (int it = threadIdx.x; it < sh.winners * each; it += LP_THREADS) {
+  const int each = (r.p.v_hi - r.p.v_lo + NT - 1) / NT + 1;  // a thread's vectors and its loose element
+  for (int it = threadIdx.x; it < sh.winners * each; it += NT) {
     const int w = sh.winner[it / each], q = it % each;
     if (q < each - 1) {
-      const int v = r.p.v_lo + w + q * LP_THREADS;
+      const int v = r.p.v_lo + w + q * NT;
       if (v >= r.p.v_hi) continue;
-      const Vec<T, PER> x = r.vec(v);
+      const uint4 raw[1] = {*reinterpret_cast<const uint4*>(r.z + r.p.head + v * PER)};
+      if (Logits<T>::largest(larger_of<T>(Logits<T>::NONE, raw)) < least) continue;
+      const Vec<T, PER> x = *reinterpret_cast<const Vec<T, PER>*>(raw);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         const uint32_t key = key_of(to_f32(x.v[j]));
@@ -317,16 +344,16 @@ __device__ int collect(const RowReader<T>& r, uint32_t from, LogprobShared& sh) 
 }
 
 // Fill up to k candidates with the first elements whose key is `key`; `have` candidates are there.
-template <typename T>
-__device__ int fill_equal(const RowReader<T>& r, int have, int k, uint32_t key, LogprobShared& sh) {
-  for (int i0 = r.p.lo; i0 < r.p.hi && have < k; i0 += LP_THREADS) {
+template <typename T, int NT>
+__device__ int fill_equal(const RowReader<T>& r, int have, int k, uint32_t key, LogprobShared<NT>& sh) {
+  for (int i0 = r.p.lo; i0 < r.p.hi && have < k; i0 += NT) {
     const int e = i0 + threadIdx.x;
     const bool is = e < r.p.hi && key_of(r.one(e)) == key;
     const unsigned who = __ballot_sync(0xffffffffu, is);
     if ((threadIdx.x & 31) == 0) sh.warp_count[threadIdx.x >> 5] = __popc(who);
     __syncthreads();
     int at = have + __popc(who & ((1u << (threadIdx.x & 31)) - 1)), all = have;
-    for (int w = 0; w < LP_THREADS / 32; ++w) {
+    for (int w = 0; w < NT / 32; ++w) {
       if (w < (int)(threadIdx.x >> 5)) at += sh.warp_count[w];
       all += sh.warp_count[w];
     }
@@ -340,15 +367,15 @@ __device__ int fill_equal(const RowReader<T>& r, int have, int k, uint32_t key, 
 // Candidates for the k largest elements: those that reach the bound. Where many may equal it (all ruled out, all alike), those
 // above it and then the first that equal it; where more lie above it than there is room for (logits in an order that puts the largest
 // into few threads' hands), the k-th largest key is found by bisection over its bits. Returns their number, k or more.
-template <typename T>
-__device__ int select_candidates(const RowReader<T>& r, int k, uint32_t own_key, LogprobShared& sh) {
+template <typename T, int NT>
+__device__ int select_candidates(const RowReader<T>& r, int k, uint32_t own_key, LogprobShared<NT>& sh) {
   constexpr uint32_t RULED_OUT = 0x007fffffu;  // the key of -inf
-  constexpr int MANY = 96;                     // threads; a bound that is not shared by many is reached by about k
+  constexpr int MANY = NT > 128 ? 96 : 48;     // threads; a bound that is not shared by many is reached by about k
   uint32_t bound = sh.bound;
   if (own_key >= bound && own_key != 0) sh.winner[atomicAdd(&sh.winners, 1)] = threadIdx.x;
   __syncthreads();
   if (bound != RULED_OUT && sh.winners <= MANY) {
-    const int n = collect(r, bound, sh);
+    const int n = collect(r, bound, value_of(bound), sh);
     if (n <= LP_CAND) return n;
   }
   auto above = [&](uint32_t key, bool mine) {  // candidates above `key`
@@ -357,7 +384,7 @@ __device__ int select_candidates(const RowReader<T>& r, int k, uint32_t own_key,
     __syncthreads();
     if (mine) sh.winner[atomicAdd(&sh.winners, 1)] = threadIdx.x;
     __syncthreads();
-    return key == 0xffffffffu ? 0 : collect(r, key + 1, sh);
+    return key == 0xffffffffu ? 0 : collect(r, key + 1, value_of(key), sh);
   };
   int n = above(bound, own_key > bound);
   if (n > LP_CAND) {
@@ -373,8 +400,9 @@ __device__ int select_candidates(const RowReader<T>& r, int k, uint32_t own_key,
 }
 
 // The `k` largest of n candidates into best[], in order (distinct keys: a place is the number of larger ones).
+template <int NT>
 __device__ __forceinline__ void rank_candidates(const unsigned long long* cand, int n, int k, unsigned long long* best) {
-  for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const unsigned long long mine = cand[i];
     int place = 0;
     for (int j = 0; j < n; ++j) place += cand[j] > mine;
@@ -414,11 +442,11 @@ __device__ __forceinline__ void write_row(const LogprobParams& a, const Sums& al
 }
 
 // `parts` CTAs (a cluster, where more than one) work on a row. Few rows are split so that more of the GPU's loads are in flight.
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 5)
+template <typename T, int NT, int CTAS>
+__global__ void __launch_bounds__(NT, CTAS)
 token_logprob_kernel(const LogprobParams a, int parts) {
   constexpr int PER = 16 / sizeof(T);
-  __shared__ LogprobShared sh;
+  __shared__ LogprobShared<NT> sh;
   grid_dep_launch();
   grid_dep_wait();
   const int rank = parts > 1 ? (int)cluster_ctarank() : 0;
@@ -430,11 +458,16 @@ token_logprob_kernel(const LogprobParams a, int parts) {
 
   // ---- the pass: sums of even and odd elements side by side in pairs, two pairs of each; the next loads are on their way
   // while these are worked on. Exponents are relative to the warp's largest logit of its first round; only one that lies LP_SLACK
-  // above (in base 2) moves that, or nearly every round some lane would, and the warp with it.
-  float top = -INFINITY;           // this thread's largest logit
-  float m = -INFINITY, mc = 0.f;  // what exponents are relative to, and times c
+  // above (in base 2; twice that where the limit's own rounding adds as much) moves that, or nearly every round some lane would, and the
+  // warp with it. Instructions bound this (3 of 4 issue slots are taken; the exponentials alone take half of their unit), so the only look
+  // at the logits' size is one comparison of packed maxima, and whole rounds know no ends of rows: 8 instructions per element became
+  // 6.5, 8192 x 50257 bf16 174 -> 166 us, 152 with 128 threads per row (5.4 TB/s), 132 without alternatives (6.2 TB/s).
+  uint32_t tops = Logits<T>::NONE;  // this thread's largest logits, in even and in odd places
+  float m = -INFINITY, mc = 0.f;    // what exponents are relative to, and times c
+  uint32_t limit = Logits<T>::word(NAN);  // above it, m moves; NaN: look at every round, there is no m yet or a huge one
   uint64_t s2[2] = {0, 0}, t2[2] = {0, 0};
   const uint64_t c2 = both_f2(a.c);
+  const float slack = LP_SLACK / a.c;
   auto raise = [&](float to) {  // (NaN stays)
     to = max_nan(m, to);
     const float d = rescale(m, to, a.c);
@@ -446,6 +479,7 @@ token_logprob_kernel(const LogprobParams a, int parts) {
     }
     m = to;
     mc = __fmul_rn(to, a.c);
+    limit = Logits<T>::word(huge(to) ? NAN : fminf(fmaxf(to, to + slack), Logits<T>::MOST));  // (rounded: m's own value at least)
   };
   auto add = [&](uint64_t d2, int i) {
     float d0, d1;
@@ -454,41 +488,46 @@ token_logprob_kernel(const LogprobParams a, int parts) {
     s2[i] = add_f2(s2[i], e2);
     t2[i] = fma_f2(e2, d2, t2[i]);
   };
-  auto work = [&](const uint4 (&v)[LP_VECS]) {
-    const float g = vec_max<T>(v);
-    top = max_nan(top, g);
-    if (huge(m) ? !(g <= m) : !(fmaf(g, a.c, -mc) <= LP_SLACK)) raise(g);
-    if (!huge(m)) {
-      const uint64_t nm2 = both_f2(-mc);
+  auto work = [&](const uint4 (&v)[LP_VECS], bool first) {
+    tops = larger_of<T>(tops, v);
+    if (Logits<T>::above(tops, limit)) {
+      float to = Logits<T>::largest(tops);
+      if (first)  // (all lanes are here)
 #pragma unroll
-      for (int u = 0; u < LP_VECS; ++u) {
-        uint64_t x[PER / 2];
-        Logits<T>::pairs(v[u], x);
+        for (int o = 16; o > 0; o >>= 1) to = max_nan(to, __shfl_xor_sync(0xffffffffu, to, o));
+      raise(to);
+      if (huge(m)) {
 #pragma unroll
-        for (int j = 0; j < PER / 2; ++j) add(fma_f2(x[j], c2, nm2), j & 1);
-      }
-    } else {
+        for (int u = 0; u < LP_VECS; ++u) {
+          const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
-      for (int u = 0; u < LP_VECS; ++u) {
-        const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+          for (int j = 0; j < 4; ++j) {
+            float x[PER / 4];
+            Logits<T>::values(w[j], x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x[PER / 4];
-          Logits<T>::values(w[j], x);
-#pragma unroll
-          for (int i = 0; i < PER / 4; ++i) add(pack_f2(fmaxf((x[i] - m) * a.c, LP_FLOOR), LP_FLOOR), 0);
+            for (int i = 0; i < PER / 4; ++i) add(pack_f2(fmaxf((x[i] - m) * a.c, LP_FLOOR), LP_FLOOR), 0);
+          }
         }
+        return;
       }
     }
+    const uint64_t nm2 = both_f2(-mc);
+#pragma unroll
+    for (int u = 0; u < LP_VECS; ++u) {
+      uint64_t x[PER / 2];
+      Logits<T>::pairs(v[u], x);
+#pragma unroll
+      for (int j = 0; j < PER / 2; ++j) add(fma_f2(x[j], c2, nm2), j & 1);
+    }
   };
-  constexpr int ROUND = LP_THREADS * LP_VECS, DEPTH = LP_RING - 1;
+  constexpr int ROUND = NT * LP_VECS, DEPTH = LP_RING - 1;
   const int vecs = r.p.v_hi - r.p.v_lo;
   const T* from = r.z + r.p.head + (r.p.v_lo + tid) * PER;  // this thread's vectors of the next round to request
-  int left = vecs - tid;                                    // > 0, > LP_THREADS, ...: as many of them exist
+  int left = vecs - tid;                                    // > 0, > NT, ...: as many of them exist
   auto request = [&](int slot) {
 #pragma unroll
     for (int u = 0; u < LP_VECS; ++u)
-      if (u * LP_THREADS < left) copy16_async(&sh.ring[slot][u][tid], from + u * (LP_THREADS * PER));
+      if (u * NT < left) copy16_async(&sh.ring[slot][u][tid], from + u * (NT * PER));
     copy_commit();
     from += ROUND * PER;
     left -= ROUND;
@@ -500,24 +539,30 @@ token_logprob_kernel(const LogprobParams a, int parts) {
   };
 #pragma unroll
   for (int i = 0; i < DEPTH; ++i) request(i);
-  const int rounds = (vecs + ROUND - 1) / ROUND;
-  for (int i = 0; i < rounds; ++i) {
+  const int rounds = (vecs + ROUND - 1) / ROUND, whole = vecs / ROUND - DEPTH;
+  int i = 0;
+  for (; i < whole; ++i) {  // rounds whose successors' requests are whole ones
+    uint4 v[LP_VECS];
+    take(i % LP_RING, v);
+#pragma unroll
+    for (int u = 0; u < LP_VECS; ++u) copy16_async(&sh.ring[(i + DEPTH) % LP_RING][u][tid], from + u * (NT * PER));
+    copy_commit();
+    from += ROUND * PER;
+    work(v, i == 0);
+  }
+  left = vecs - tid - (i + DEPTH) * ROUND;
+  for (; i < rounds; ++i) {
     uint4 v[LP_VECS];
     take(i % LP_RING, v);
     if (i + 1 == rounds) {  // vectors that do not exist
 #pragma unroll
       for (int u = 0; u < LP_VECS; ++u)
-        if (i * ROUND + u * LP_THREADS + tid >= vecs) v[u] = make_uint4(Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE);
+        if (i * ROUND + u * NT + tid >= vecs) v[u] = make_uint4(Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE);
     }
     request((i + DEPTH) % LP_RING);
-    if (i == 0) {
-      float first = vec_max<T>(v);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) first = max_nan(first, __shfl_xor_sync(0xffffffffu, first, o));
-      raise(first);
-    }
-    work(v);
+    work(v, i == 0);
   }
+  float top = Logits<T>::largest(tops);
   Sums sum;
   {
     float s0, s1, t0, t1;
@@ -537,32 +582,38 @@ token_logprob_kernel(const LogprobParams a, int parts) {
   const bool nothing = tid >= r.p.v_hi - r.p.v_lo && single < 0;
   const uint32_t own_key = nothing ? 0u : key_of(top);
   if (k > 0) {
-    // groups of 4 threads; of 2 or 1 where there are no more vectors than that makes groups
-    const int share = r.p.v_hi - r.p.v_lo > 2 * LP_GROUPS ? 4 : r.p.v_hi - r.p.v_lo > LP_GROUPS ? 2 : 1;
+    // groups of 4 threads (of 256); of 2 or 1 where there are no more vectors than that makes groups
+    int share = 1;
+    while (share * LP_GROUPS < NT && r.p.v_hi - r.p.v_lo > share * LP_GROUPS) share *= 2;
     uint32_t g = own_key;
     if (share > 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, 1));
     if (share > 2) g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
     if (tid % share == 0 && tid / share < LP_GROUPS) sh.group[tid / share] = g;
     if (tid < LP_TOP) sh.best[tid] = 0;
-    if (tid == 0) sh.winners = sh.found = 0;
+    if (tid == 0) sh.winners = sh.found = 0, sh.bound = 0xffffffffu;
   }
   sum = join_lanes<32>(sum, a.c);
   if (lane == 0) sh.part[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    sum = join_lanes<LP_THREADS / 32>(sh.part[lane % (LP_THREADS / 32)], a.c);
+    sum = join_lanes<NT / 32>(sh.part[lane % (NT / 32)], a.c);
     if (parts > 1 && lane == 0) sh.all = sum;
   }
   if (k > 0) {
-    if (tid < LP_GROUPS) {
+    if (tid < LP_GROUPS) {  // the smallest of those that fewer than k are larger than
       const uint32_t g = sh.group[tid];
-      int place = 0;
-      for (int j = 0; j < LP_GROUPS; ++j) place += sh.group[j] > g || (sh.group[j] == g && j < tid);
-      if (place == k - 1) sh.bound = g;
+      int larger = 0;
+#pragma unroll
+      for (int j = 0; j < LP_GROUPS; j += 4) {
+        const uint4 o = *reinterpret_cast<const uint4*>(sh.group + j);
+        larger += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
+      }
+      const uint32_t b = __reduce_min_sync(0xffffffffu, larger < k ? g : 0xffffffffu);
+      if (lane == 0) atomicMin(&sh.bound, b);
     }
     __syncthreads();
     const int n = select_candidates(r, k, own_key, sh);
-    rank_candidates(sh.cand, n, k, sh.best);
+    rank_candidates<NT>(sh.cand, n, k, sh.best);
     __syncthreads();
   }
 
@@ -578,14 +629,14 @@ token_logprob_kernel(const LogprobParams a, int parts) {
         all = join(all, other, a.c);
       }
       if (a.top > 0) {
-        for (int i = tid; i < parts * a.top; i += LP_THREADS) {
+        for (int i = tid; i < parts * a.top; i += NT) {
           const int q = i / a.top, j = i - q * a.top;
           sh.cand[i] = q == 0 ? sh.best[j] : cluster_load64(&sh.best[j], q);
         }
         __syncthreads();
         if (tid < LP_TOP) sh.best[tid] = 0;
         __syncthreads();
-        rank_candidates(sh.cand, parts * a.top, a.top, sh.best);
+        rank_candidates<NT>(sh.cand, parts * a.top, a.top, sh.best);
         __syncthreads();
       }
     }
@@ -699,11 +750,17 @@ int tnnb_token_logprob(const void* z, long long ld, const void* tokens, int toke
   while (parts < LP_CLUSTER && rows * parts * 2 <= 148 && bytes / parts >= 48 << 10) parts *= 2;
   const LogprobParams p = {z, ld, tokens, tokens64, rows, V, top, c, ignore, (float*)logp, (float*)entropy, (float*)top_logp,
                            (long long*)top_index, (float*)stats};
+  // What a row costs beside its elements (statistics joined, alternatives found) is per warp, so a CTA has few of them where rows fill
+  // the GPU all the same. Us with 64, 128 and 256 threads, alternatives included: 20000 x 2000 bf16 71, 105, 176; 1000 x 8000 bf16 14.4,
+  // 12.5, 16.5; 10000 x 8000 62, 72, 105; 8192 x 50257 bf16 207, 152, 168; 999 x 128001 fp32 183, 122, 103; 2048 of those 386, 237, 199.
+  const int threads = bytes < (rows < 148 * 20 ? 8 << 10 : 16 << 10) ? 64 : bytes < (rows < 148 * 8 ? 32 << 10 : 192 << 10) ? 128 : 256;
   cudaError_t e = cudaSuccess;
   const bool known = with_type(type, [&](auto tag) {
     using T = typename decltype(tag)::type;
-    auto kern = token_logprob_kernel<T>;
-    e = launch_dependent_cluster(kern, parts, dim3((unsigned)(rows * parts)), dim3(LP_THREADS), 0, (cudaStream_t)stream, p, parts);
+    auto kern = threads == 64    ? token_logprob_kernel<T, 64, 20>
+                : threads == 128 ? token_logprob_kernel<T, 128, 8>
+                                 : token_logprob_kernel<T, 256, sizeof(T) == 4 ? 4 : 5>;
+    e = launch_dependent_cluster(kern, parts, dim3((unsigned)(rows * parts)), dim3(threads), 0, (cudaStream_t)stream, p, parts);
   });
   if (!known) return -4;
   return e == cudaSuccess ? 0 : -(int)e - 1000;
