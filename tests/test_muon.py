@@ -248,3 +248,19 @@ def test_places_on_another_device_are_refused():
         raw.muon_momentum(torch.zeros(24, device="cuda"), group, torch.zeros(1, 4, 6, device="cuda"), 0.9)
     with pytest.raises(ValueError):
         raw.muon_apply(torch.zeros(24, device="cuda"), None, group, torch.zeros(1, 4, 6, device="cuda", dtype=torch.bfloat16), 0.1, 1.0)
+
+
+def test_replicas_reduced_by_the_library():
+    """The update of data-parallel replicas that all-reduce their gradients: scaled by a power of two, the same bits."""
+    from tnn_b200.parallel import dp
+
+    g1, g2 = (zoo.gpt2(64, 1, 1, "t", seq_len=8, vocab=20).compile(device="cpu", seed=0) for _ in range(2))
+    one = dp.NcclDPOptimizer(Muon(0.01), g1, [dp.Region(0, g1.total_elems, [0], None)], 0.5)
+    two = Muon(0.01).attach(g2)
+    for k in range(2):
+        grads = torch.randn(g1.total_elems, generator=torch.Generator().manual_seed(k))
+        g1.grads_flat.copy_(grads)
+        g2.grads_flat.copy_(grads * 0.5)
+        one.update()
+        two.update()
+    assert torch.equal(g1.master_flat, g2.master_flat)

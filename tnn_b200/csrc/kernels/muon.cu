@@ -5,7 +5,7 @@
 //   w <- w - lr (factor o + decay w)    with o = the orthogonalised u, in bf16
 //
 // Weights and gradients lie in flat buffers at given offsets, equal matrices are one launch; state and updates are packed. One pass
-// over the bytes each: bound by memory. The learning rate and the gradients' scale may come from device memory (`hyper`, as for the other
+// over the bytes each: bound by memory (four fp32 and three fp32 and bf16 streams). The learning rate and the gradients' scale may come from device memory (`hyper`, as for the other
 // optimizers), so that a captured step sees new ones.
 #include "ptx.cuh"
 #include "values.cuh"

@@ -648,7 +648,7 @@ token_logprob_kernel(const LogprobParams a, int parts) {
 
 // ---------------------------------------------------------------------------------------------------------- gradient
 // dz_j = p_j (A + B d_j) with d_j = log2 p_j, A = -(g + h H) / temperature, B = -h ln 2 / temperature, and g / temperature more at the
-// token. One read, one write.
+// token. One read, one write, bound by memory: 4096 x 50257 bf16 140 us, 5.9 TB/s.
 struct LogprobGradParams {
   const void* z;
   long long ld;
