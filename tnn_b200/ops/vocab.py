@@ -66,7 +66,7 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
 
 
 def _new(like: torch.Tensor, dtype, *sizes: int) -> torch.Tensor:
-    return _lib.empty(like, dtype, *sizes) if len(sizes) <= 8 else torch.empty(sizes, dtype=dtype, device=like.device)
+    return torch.empty(sizes, dtype=dtype, device=like.device)  # (_lib.empty takes eight dimensions)
 
 
 def _pitch(t: torch.Tensor) -> int:
@@ -89,7 +89,7 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         code = _type_code(table, "embedding table")
         table = _rows(table, width)
         with _lib.device_of(table):
-            out = _new(table, table.dtype, *ids.shape, width)
+            out = _lib.empty(table, *ids.shape, width) if ids.dim() < 8 else _new(table, table.dtype, *ids.shape, width)
             if n:
                 rc = _library().tnnb_embed_lookup(flat, flat.dtype is torch.int64, table.data_ptr(), max(_pitch(table), width), out, n, width, rows, pad,
                                                   float(scale), code, _lib.raw_stream())
@@ -205,8 +205,9 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
         code = _type_code(logits, "logits")
         with _lib.device_of(z):
             f32 = torch.float32
-            lp, ent = _new(z, f32, *shape), _new(z, f32, *shape)
-            top, idx = _new(z, f32, *shape, top_k), _new(z, torch.int64, *shape, top_k)
+            new = _lib.empty if len(shape) < 8 else _new
+            lp, ent = new(z, f32, *shape), new(z, f32, *shape)
+            top, idx = new(z, f32, *shape, top_k), new(z, torch.int64, *shape, top_k)
             stats = _lib.empty(z, f32, rows, 2) if keep is not None else None
             if rows:
                 rc = _library().tnnb_token_logprob(z.data_ptr(), max(_pitch(z), V), tok, tok.dtype is torch.int64, lp, ent, top, idx, stats, rows, V, top_k,
