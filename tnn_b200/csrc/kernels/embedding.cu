@@ -65,10 +65,11 @@ embed_lookup_kernel(const ID* __restrict__ ids, const T* __restrict__ table, lon
 //
 // Rows are dealt out in turn (2^bits CTAs; row v is number v >> bits of CTA v mod 2^bits): frequent tokens have neighbouring numbers, and
 // with ranges of rows the CTA that had them took 16 us for 8192 tokens of text, 63 for 50001. The list is in this order of rows
-// ("slots"), which is as good as any. Looking twice at every position cost 10 us of 97 for 50001 positions of 1001 fp32 columns.
+// ("slots"), which is as good as any. Looking twice at every position cost 17 us of 97 for 50001 positions
+// of 1001 fp32 columns.
 static constexpr int SORT_WARPS = 32;
 static constexpr int SORT_ROWS = 512;  // most rows of a CTA, one per thread
-static constexpr int SORT_NOTES = 128;  // positions that a warp notes: row in 9 bits, place in its stretch in 23
+static constexpr int SORT_NOTES = 512;  // most positions that a warp notes: row in 9 bits, place in its stretch in 23
 static constexpr uint32_t TOKEN_FIRST = 1u << 30, TOKEN_LAST = 1u << 31, TOKEN_ROW = TOKEN_FIRST - 1;
 
 struct Slots {
@@ -82,6 +83,7 @@ __host__ __device__ __forceinline__ Slots slots_of(long long vocab) {
   s.rows = (int)((vocab + (1ll << s.bits) - 1) >> s.bits);
   return s;
 }
+__host__ __device__ __forceinline__ int sort_stretch(int n) { return (int)(((n + SORT_WARPS - 1ll) / SORT_WARPS + 127) / 128 * 128); }  // positions of a warp
 __device__ __forceinline__ int slot_of(const Slots& s, int row) { return (row & ((1 << s.bits) - 1)) * s.rows + (row >> s.bits); }
 
 // A position's CTA and the row's number there, 16 bits each (NO_CODE: padding). Every CTA looks at every position twice: what it
@@ -101,20 +103,20 @@ embed_code_kernel(const ID* ids, int n, long long vocab, long long padding, Slot
 }
 
 __global__ void __launch_bounds__(SORT_WARPS * 32)
-embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_t* keys, int* rowptr) {
-  extern __shared__ int counters[];  // [SORT_WARPS][slots.rows]
+embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int room, int* order, uint32_t* keys, int* rowptr) {
+  extern __shared__ int counters[];  // [SORT_WARPS][slots.rows], [SORT_WARPS][room] notes
   __shared__ int below[SORT_WARPS], scan[SORT_WARPS];
   __shared__ int begin[SORT_ROWS], count[SORT_ROWS];
-  __shared__ uint32_t notes[SORT_WARPS][SORT_NOTES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = slots.rows, own = blockIdx.x, mask = (1 << slots.bits) - 1;
   for (int i = threadIdx.x; i < SORT_WARPS * rows; i += blockDim.x) counters[i] = 0;
   grid_dep_wait();
   __syncthreads();
 
-  const int stretch = ((n + SORT_WARPS - 1) / SORT_WARPS + 127) / 128 * 128;  // of a warp
+  const int stretch = sort_stretch(n);
   const int lo = min((long long)n, (long long)warp * stretch), hi = min((long long)n, (long long)lo + stretch);
   int* mine = counters + warp * rows;
+  uint32_t* notes = reinterpret_cast<uint32_t*>(counters) + SORT_WARPS * rows + warp * room;
   const uint32_t base = (uint32_t)own << 16;
   // Calls f(four codes, place of the first) for the warp's positions, 128 at a time; the next ones are on their way meanwhile. (`codes`
   // begins on 16 bytes and ends on a whole vector.)
@@ -140,7 +142,7 @@ embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_
       }
     }
   };
-  int less = 0, noted = stretch < 1 << 23 ? 0 : SORT_NOTES + 1;
+  int less = 0, noted = stretch < 1 << 23 ? 0 : room + 1;
   walk([&](const uint32_t (&w)[4], int position) {
     bool any = false;
 #pragma unroll
@@ -156,9 +158,9 @@ embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_
       const int at = noted + __popc(who & ((1u << lane) - 1));
       if (in) {
         atomicAdd(&mine[w[j] & 0xffffu], 1);
-        if (at < SORT_NOTES) notes[warp][at] = (w[j] & 0xffffu) << 23 | (uint32_t)(position + j - lo);
+        if (at < room) notes[at] = (w[j] & 0xffffu) << 23 | (uint32_t)(position + j - lo);
       }
-      noted = min(noted + __popc(who), SORT_NOTES + 1);  // (one more: there was no room)
+      noted = min(noted + __popc(who), room + 1);  // (one more: there was no room)
     }
   });
 #pragma unroll
@@ -213,9 +215,9 @@ embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_
     }
     __syncwarp();
   };
-  if (noted <= SORT_NOTES) {
+  if (noted <= room) {
     for (int i = lane; i - lane < noted; i += 32) {
-      const uint32_t note = i < noted ? notes[warp][i] : 0u;
+      const uint32_t note = i < noted ? notes[i] : 0u;
       place(i < noted, (int)(note >> 23), lo + (int)(note & 0x7fffffu));
     }
   } else {
@@ -236,7 +238,7 @@ embed_sort_kernel(const uint32_t* codes, int n, Slots slots, int* order, uint32_
 //
 // A thread has COLS vectors of VEC columns, blockDim.x vectors apart (single columns where rows are not aligned: four of them share
 // the bookkeeping). Bound by memory, behind four kernels in a row: all of it 31 us for 8192 x 768 bf16 and 50257 rows (90 MB; 21 of them
-// without the clearing), 86 us for 50001 x 1001 fp32 and 32003 rows (329 MB, 60 of them here). Clearing beside the sort, which
+// without the clearing), 80 us for 50001 x 1001 fp32 and 32003 rows (329 MB, 58 of them here). Clearing beside the sort, which
 // needs a mark per row, is no faster (34 and 99 us, as stores or as bulk copies): the sorting CTAs' loads then wait behind the writes.
 __device__ __forceinline__ void clear_row(uint8_t* row, long long bytes, int lane) {  // one warp; addresses are even
   const int head = (int)min(bytes, (long long)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15));
@@ -245,6 +247,22 @@ __device__ __forceinline__ void clear_row(uint8_t* row, long long bytes, int lan
   for (long long i = lane; i < body; i += 32) reinterpret_cast<uint4*>(row + head)[i] = make_uint4(0, 0, 0, 0);
   const long long tail = head + body * 16 + lane * 2;
   if (tail < bytes) *reinterpret_cast<uint16_t*>(row + tail) = 0;
+}
+
+// p[j] += v[j] * scale, N of them, by the memory: nobody else adds to them meanwhile, so the order is fixed, and nothing waits for the
+// old value (with a load and a store a CTA spent a round trip on every token, 46 us for 32768 x 768 bf16).
+template <int N>
+__device__ __forceinline__ void add_to(float* p, const float (&v)[N], float scale) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4)
+      asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + j), "f"(v[j] * scale), "f"(v[j + 1] * scale),
+                   "f"(v[j + 2] * scale), "f"(v[j + 3] * scale)
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(p + j), "f"(v[j] * scale) : "memory");
+  }
 }
 
 template <typename TI, typename TO, int VEC, int COLS>
@@ -317,12 +335,16 @@ embed_sum_kernel(const TI* dy, long long ld, const int* order, const uint32_t* k
 #pragma unroll
         for (int c = 0; c < COLS; ++c) {
           if (col0 + c * step >= width) continue;
-          Vec<TO, VEC>* at = reinterpret_cast<Vec<TO, VEC>*>(o + col0 + c * step);
+          if constexpr (sizeof(TO) == 4) {
+            if (accumulate) {
+              add_to<VEC>(reinterpret_cast<float*>(o) + col0 + c * step, sum[c], scale);
+              continue;
+            }
+          }
           Vec<TO, VEC> r;
-          if (accumulate) r = *at;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) r.v[j] = from_f32<TO>(accumulate ? to_f32(r.v[j]) + sum[c][j] * scale : sum[c][j] * scale);
-          *at = r;
+          for (int j = 0; j < VEC; ++j) r.v[j] = from_f32<TO>(sum[c][j] * scale);
+          *reinterpret_cast<Vec<TO, VEC>*>(o + col0 + c * step) = r;
         }
       }
       from_before = false;
@@ -406,10 +428,11 @@ static cudaError_t sort_tokens(const void* ids, int n, long long vocab, long lon
   auto code = embed_code_kernel<ID>;
   cudaError_t e = launch_dependent(code, dim3((n + 255) / 256), dim3(256), 0, st, (const ID*)ids, n, vocab, padding, slots, codes);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_WARPS * SORT_ROWS * (int)sizeof(int));
+  e = cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_WARPS * (SORT_ROWS + SORT_NOTES) * (int)sizeof(int));
   if (e != cudaSuccess) return e;
-  return launch_dependent(embed_sort_kernel, dim3(1u << slots.bits), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * slots.rows * sizeof(int), st,
-                          (const uint32_t*)codes, n, slots, order, keys, rowptr);
+  const int stretch = sort_stretch(n), room = stretch < SORT_NOTES ? stretch : SORT_NOTES;
+  return launch_dependent(embed_sort_kernel, dim3(1u << slots.bits), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * (slots.rows + room) * sizeof(int), st,
+                          (const uint32_t*)codes, n, slots, room, order, keys, rowptr);
 }
 
 }  // namespace tnnb
