@@ -5,7 +5,8 @@
 // (matrices with more rows than columns: A = X^T X and X <- a X + X B). Each step pulls the singular values towards one.
 //
 // All products of all steps run in ONE kernel on the tcgen05 tensor cores. What the mathematics gives away is used:
-//   * A and B are symmetric: tiles on and above the diagonal are computed, the others stored as their transposes;
+//   * A and B are symmetric: tiles on and above the diagonal are computed; the others are read as those, across, or stored as their
+//     transposes;
 //   * b A and a X are added in the epilogues, nothing is materialised but A, B and X;
 //   * neither orientation needs a transposed copy: the operands of X X^T, X^T X, B X and X B are the stored matrices, K-major or
 //     MN-major;
@@ -24,7 +25,7 @@
 // Figures (five steps; floor: the products with their symmetry at the measured bf16 rate). 12 x 2304 x 768 fp32 413 - 485 us (167) by the
 // clock that the power limit leaves, 48 of them the two passes of the norm, 8 x 1280 x 5120 bf16 1200 - 1400 (670): a K block of a CTA
 // pair takes 0.38 to 0.46 us, the rate of the library's products, the rest is what no tile overlaps (a product's last round, epilogues
-// with two addends). One 768 x 768 matrix 125 us (6), 9 x 321 x 1155 176 (11): fifteen products in a row, each 1 us to the first
+// with two addends). One 768 x 768 matrix 124 us (6), 9 x 321 x 1155 168 (11): fifteen products in a row, each 1 us to the first
 // copy, 0.3 us per K block (what one SM gets out of L2, 80 GB/s), 0.6 to 1.6 us of epilogue and 1.9 us until the next
 // product has seen it.
 #include <cuda_fp16.h>
@@ -109,6 +110,22 @@ __device__ __forceinline__ NsTask ns_task(const NsParams& p, long long work) {
     t.nb = RATIO * t.mb + k;
   }
   return t;
+}
+
+// How a tile's operands lie in memory: the first `a` K blocks of A's operand and the first `b` of B's are MN-major. X's all are or none;
+// of a symmetric matrix those left of the diagonal tile that its rows meet, where they are stored across only. (CTA pairs store both
+// triangles: reading across saves an epilogue its transposed stores, 127 and 124 us for one 768 x 768, 175 and 168 for 9 x 321 x 1155, but
+// MN-major operands cost a busy tensor pipe more than that, 8 x 1280 x 5120 1215 and 1270.)
+struct NsTurns {
+  int a, b;
+};
+template <int PAIR, int TM, int BN, int TALL>
+__device__ __forceinline__ NsTurns ns_turns(const NsTask& t) {
+  constexpr int ALL = 1 << 30;
+  const int a = PAIR ? 0 : t.mb * (TM / 64), b = PAIR ? 0 : t.nb * BN / TM * (TM / 64);
+  if (t.phase == NS_GRAM) return TALL ? NsTurns{ALL, ALL} : NsTurns{0, 0};
+  if (t.phase == NS_POLY) return {a, b};
+  return TALL ? NsTurns{0, b} : NsTurns{a, ALL};
 }
 
 // Waits until the product that `t` reads is complete (the one before it, of the same matrix). Called by one lane.
@@ -417,7 +434,7 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
         const int x = t.step & 1;
         const CUtensorMap* ma = t.phase == NS_POLY ? &maps.gram : t.phase == NS_STEP && !TALL ? &maps.poly : &maps.x[x];
         const CUtensorMap* mb = t.phase == NS_POLY ? &maps.gram : t.phase == NS_STEP && TALL ? &maps.poly : &maps.x[x];
-        const bool a_mn = TALL && t.phase == NS_GRAM, b_mn = t.phase == NS_GRAM ? TALL : (t.phase == NS_STEP && !TALL);
+        const NsTurns turns = ns_turns<PAIR, TM, BN, TALL>(t);
         const int row0 = t.mb * TM + rank * 128, col0 = t.nb * BN + rank * (BN / 2);  // this CTA's rows of A and of B
         const int k_blocks = t.phase == NS_GRAM ? p.k_gram : p.k_rest;
         fence_proxy_async_all();  // what other SMs have stored is visible to the copies that follow
@@ -429,6 +446,7 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
           }
           uint8_t* a_dst = smem + stage * Cfg::STAGE;
           uint8_t* b_dst = a_dst + Cfg::A_BYTES;
+          const bool a_mn = PAIR ? turns.a != 0 : kb < turns.a, b_mn = PAIR ? turns.b != 0 : kb < turns.b;
           if (rank == 0) mbar_expect_tx(&full[stage], (1 + PAIR) * Cfg::STAGE);
           if (PAIR) {
             const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
@@ -482,8 +500,7 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
           break;
         }
         mbar_arrive(&ring.empty[i % NS_RING]);
-        const int a_mn = TALL && t.phase == NS_GRAM, b_mn = t.phase == NS_GRAM ? TALL : (t.phase == NS_STEP && !TALL);
-        const uint32_t idesc = make_idesc_f16(TM, BN, a_mn, b_mn);
+        const NsTurns turns = ns_turns<PAIR, TM, BN, TALL>(t);
         const int k_blocks = t.phase == NS_GRAM ? p.k_gram : p.k_rest;
         if (!wait_or_abort(&tempty[acc], acc_phase ^ 1, abort_flag)) {
           ns_give_up(p, abort_flag, ST_TIMEOUT_MMA);
@@ -501,6 +518,8 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
             break;
           }
           tc_fence_after();
+          const int a_mn = PAIR ? turns.a != 0 : kb < turns.a, b_mn = PAIR ? turns.b != 0 : kb < turns.b;
+          const uint32_t idesc = make_idesc_f16(TM, BN, a_mn, b_mn);
           const uint32_t a_addr = smem_u32(smem + stage * Cfg::STAGE), b_addr = a_addr + Cfg::A_BYTES;
           const uint64_t ad0 = a_mn ? make_smem_desc(a_addr, 8192, 1024) : make_smem_desc(a_addr, 16, 1024);
           const uint64_t bd0 = b_mn ? make_smem_desc(b_addr, 8192, 1024) : make_smem_desc(b_addr, 16, 1024);
@@ -560,7 +579,7 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
       const bool folded = t.step + NS_FOLDED >= p.steps, last = t.step + 1 == p.steps;
       const float a = p.coef[3 * t.step], b = p.coef[3 * t.step + 1], c = p.coef[3 * t.step + 2];
       const int row0 = t.mb * TM + rank * 128 + q * 32, col0 = t.nb * BN + wcol;
-      const bool mirror = t.nb >= RATIO * (t.mb + 1);
+      const bool mirror = PAIR && t.nb >= RATIO * (t.mb + 1);
       const uint32_t t_addr = tmem_base + acc * BN + (static_cast<uint32_t>(q * 32) << 16) + wcol;
       const auto wait_full = [&] {
         bool there = wait_or_abort(&tfull[acc], acc_phase, abort_flag);
