@@ -616,8 +616,7 @@ ns_products_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ 
       if (!(last && t.phase == NS_STEP)) {  // the warp's part of the tile is there for everyone
         __syncwarp();
         if (lane == 0) {
-          __threadfence();
-          atomicAdd(p.done + (long long)(3 * t.step + t.phase) * p.items + t.item, 1u);
+          asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.done + (long long)(3 * t.step + t.phase) * p.items + t.item) : "memory");
         }
       }
       acc ^= 1;
