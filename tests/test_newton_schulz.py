@@ -185,3 +185,13 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(x, alone[i]) for x in got[i])
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    far = 2 ** 31 + 16  # elements between two matrices, and between two rows of one
+    space = torch.empty(far + 4096, dtype=torch.bfloat16, device="cuda")
+    for shape, strides in (((2, 20, 30), (far, 30, 1)), ((2, 30), (far, 1))):
+        g = space.as_strided(shape, strides)
+        g.copy_(torch.randn(shape))
+        assert torch.equal(raw.newton_schulz(g), raw.newton_schulz(g.contiguous()))

@@ -334,3 +334,20 @@ def test_rows_of_every_length_agree(rows, vocab):
     tol_lp, tol_ent = _tolerances(z[some], tokens[some], lp, ent, vocab, 1.0)
     within(many.log_probs[some.cuda()], lp, tol_lp)
     within(many.entropy[some.cuda()], ent, tol_ent)
+
+
+def test_offsets_beyond_32_bits():
+    far = 2 ** 31 + 16  # elements between two rows
+    space = torch.empty(far + 1024, dtype=torch.bfloat16, device="cuda")
+    rows = space.as_strided((2, 1000), (far, 1))
+    rows.copy_(torch.randn(2, 1000))
+    near = rows.contiguous()
+    ids = torch.tensor([1, 0, 1], device="cuda")
+    assert torch.equal(raw.embedding_lookup(ids, rows, 2.0), raw.embedding_lookup(ids, near, 2.0))
+    one = torch.tensor([0, 1], device="cuda")
+    assert torch.equal(raw.embedding_grad(one, rows, 3), raw.embedding_grad(one, near, 3))
+    kept, plain = {}, {}
+    a, b = raw.token_log_probs(rows, one, 4, keep=kept), raw.token_log_probs(near, one, 4, keep=plain)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    g = torch.randn(2, device="cuda")
+    assert torch.equal(raw.token_log_probs_grad(rows, one, kept, g, g), raw.token_log_probs_grad(near, one, plain, g, g))
