@@ -81,6 +81,13 @@ def test_embedding_gradient(dtype, n, vocab, width, kind):
     assert torch.equal(acc.cpu()[untouched], base[untouched])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,vocab,width", [(2, 70001, 8), (31, 500, 1027), (33, 8, 2056), (127, 100, 300), (128, 700, 96), (129, 700, 96), (128, 3, 1030)])
+@pytest.mark.parametrize("kind", ["zipf", "one", "uniform"])
+def test_embedding_gradient_of_few_positions(dtype, n, vocab, width, kind):
+    test_embedding_gradient(dtype, n, vocab, width, kind)
+
+
 def test_embedding_gradient_of_views_and_large_vocabularies():
     n, vocab, width = 500, 200_003, 16  # more rows than two CTAs per SM hold at 512 each
     ids = ids_for(n, vocab, "uniform", 4)

@@ -104,6 +104,9 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     return out.to(table.dtype).view(*ids.shape, width)
 
 
+_FEW = 128  # positions whose gradient is one kernel without workspaces (embedding.cu's EMBED_FEW)
+
+
 def _chunk(n: int) -> int:
     """Sorted positions per CTA of the gradient's sums: enough CTAs for the SMs (148, several on each), and no more parts of tokens
     that lie in several chunks than that takes."""
@@ -143,17 +146,24 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
         with _lib.device_of(dy2):
             if out is None:
                 out = _lib.empty(dy2, rows, width)
+            pitch = max(_pitch(dy2), width) if n else width
+            if n <= _FEW:
+                rc = _library().tnnb_embed_grad(flat, flat.dtype is torch.int64, dy2, pitch, out, None, None, None, None, None, n, width, rows, pad,
+                                                float(scale), code, _TYPES[out.dtype], int(accumulate), 16, _lib.raw_stream())
+                _lib.check_rc(rc, "embedding_grad")
+                LAUNCHES["count"] += 1 if n else 0
+                return out
             chunk = _chunk(n)
             # where each position belongs, sorted positions and their tokens, where each row's begin; partial sums of tokens in several chunks
             n4 = (n + 3) // 4 * 4
             ints = _lib.empty(dy2, torch.int32, n4 + 2 * n + rows + rows // 256 + 129)
             parts = _lib.empty(dy2, torch.float32, 2 * ((n + chunk - 1) // chunk) * width)
             base = ints.data_ptr()
-            rc = _library().tnnb_embed_grad(flat, flat.dtype is torch.int64, dy2, max(_pitch(dy2), width) if n else width, out, base,
-                                            base + 4 * n4, base + 4 * (n4 + n), base + 4 * (n4 + 2 * n), parts, n, width, rows, pad, float(scale), code, _TYPES[out.dtype],
+            rc = _library().tnnb_embed_grad(flat, flat.dtype is torch.int64, dy2, pitch, out, base, base + 4 * n4, base + 4 * (n4 + n),
+                                            base + 4 * (n4 + 2 * n), parts, n, width, rows, pad, float(scale), code, _TYPES[out.dtype],
                                             int(accumulate), chunk, _lib.raw_stream())
             _lib.check_rc(rc, "embedding_grad")
-            LAUNCHES["count"] += 4 if n > chunk else 3
+            LAUNCHES["count"] += 4
         return out
     flat = flat.reshape(-1)
     safe = torch.where((flat < 0) | (flat >= rows), torch.zeros_like(flat), flat).long()
