@@ -48,7 +48,8 @@ def off(got, ref):
 ROUNDED = 2.0 ** -8 / math.sqrt(3)
 # fp16 operands: a product's operands are off by at most 2^-11 each, root mean square 2^-11 / sqrt(3) = 0.00028. In a step three roundings
 # reach X (of X in A and in B X, of A, of B), each times coefficients of size |b| sigma^2 + 2 |c| sigma^4 < 8 at most; errors of
-# earlier steps are multiplied by the quintic's slope, which is above one only while the matrix grows by the same factor, so that five steps
+# earlier steps are multiplied by the quintic's slope, which is above one while the matrix grows by the same factor (and near singular
+# values of 1.2, up to 3.9, which few of a matrix's are: not so where a matrix has only a few), so that five steps
 # add up to at most sqrt(5 * 4) * 8 / 2 (the mean of sigma^2 over the steps is below 1/2) times that.
 OPERANDS = 2.0 ** -11 / math.sqrt(3) * math.sqrt(20) * 4
 BOUND = ROUNDED + OPERANDS
