@@ -171,13 +171,16 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
 
-// Logits from here on might overflow when they are multiplied by c. Numbers of that size differ by far more than any exponent, so
-// that (z - m) c, which loses the digits below theirs, is as good there; elsewhere z c - m c, one fused operation, is better: the
-// rounding of m c is common to all terms of a row.
-__device__ __forceinline__ bool huge(float m) { return !(fabsf(m) < 1e20f); }
+// Exponents relative to a logit m are z c - (m c rounded), one fused operation per element: what is rounded off m c is common to all terms
+// of a row. It must stay small, or the whole row's sum overflows or vanishes with it: up to 2^24 it is half a unit at most. From there
+// on (rows filled with a finite mask value, small temperatures, infinities, NaN) exponents are (z - m) c: logits that are not within a
+// factor of two of m have no probability left, and for the others the difference is exact.
+__device__ __forceinline__ bool huge(float m, float c) { return !(fabsf(__fmul_rn(m, c)) < 16777216.f); }
+// What exponents relative to m are too large by.
+__device__ __forceinline__ float excess(float m, float c) { return huge(m, c) ? 0.f : fmaf(m, c, -__fmul_rn(m, c)); }
 // The exponent of one maximum relative to another, 0 for equal ones.
 __device__ __forceinline__ float rescale(float m, float to, float c) {
-  const float d = huge(m) || huge(to) ? (m - to) * c : __fmul_rn(m, c) - __fmul_rn(to, c);
+  const float d = huge(m, c) || huge(to, c) ? (m - to) * c - excess(m, c) + excess(to, c) : __fmul_rn(m, c) - __fmul_rn(to, c);
   return fmaxf(d, LP_FLOOR);
 }
 
@@ -420,7 +423,7 @@ __device__ __forceinline__ void write_row(const LogprobParams& a, const Sums& al
   auto log_prob = [&](float v) -> float {
     if (bad) return NAN;
     if (dead || v == -INFINITY) return -INFINITY;
-    const double d = huge(all.m) ? ((double)v - all.m) * a.c : (double)v * a.c - __fmul_rn(all.m, a.c);
+    const double d = huge(all.m, a.c) ? ((double)v - all.m) * a.c : (double)v * a.c - __fmul_rn(all.m, a.c);
     return (float)((d - ls) * ln2);
   };
   if (lane < a.top) {
@@ -479,7 +482,7 @@ token_logprob_kernel(const LogprobParams a, int parts) {
     }
     m = to;
     mc = __fmul_rn(to, a.c);
-    limit = Logits<T>::word(huge(to) ? NAN : fminf(fmaxf(to, to + slack), Logits<T>::MOST));  // (rounded: m's own value at least)
+    limit = Logits<T>::word(huge(to, a.c) ? NAN : fminf(fmaxf(to, to + slack), Logits<T>::MOST));  // (rounded: m's own value at least)
   };
   auto add = [&](uint64_t d2, int i) {
     float d0, d1;
@@ -496,7 +499,7 @@ token_logprob_kernel(const LogprobParams a, int parts) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) to = max_nan(to, __shfl_xor_sync(0xffffffffu, to, o));
       raise(to);
-      if (huge(m)) {
+      if (huge(m, a.c)) {
 #pragma unroll
         for (int u = 0; u < LP_VECS; ++u) {
           const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
@@ -572,7 +575,7 @@ token_logprob_kernel(const LogprobParams a, int parts) {
   }
   const int single = loose<T>(r.p, tid);
   if (single >= 0) {
-    const float z = r.one(single), d = huge(z) ? 0.f : fmaf(z, a.c, -__fmul_rn(z, a.c)), e = exp2f(d);  // as in the pass: z c - (z c rounded)
+    const float z = r.one(single), d = excess(z, a.c), e = exp2f(d);  // as in the pass
     sum = join(sum, {z, e, e * d}, a.c);
     top = max_nan(top, z);
   }
@@ -688,11 +691,11 @@ token_logprob_grad_kernel(const LogprobGradParams a) {
     for (int j = part * 256 + threadIdx.x; j < a.V; j += a.splits * 256) dz[j] = v;
     return;
   }
-  // log2 p = (x - m) c - (log2 s, less what the rounding of m c took off the sum's exponents)
-  const float off = fmaf(m, a.c, -__fmul_rn(m, a.c)) - ls;
-  const bool big = huge(m);
+  // log2 p = (x - m) c - (log2 s, less what the sum's exponents are too large by)
+  const float off = excess(m, a.c) - ls;
+  const bool big = huge(m, a.c);
   auto one = [&](float x, int j) {
-    const float d = fmaxf(fmaf(x - m, a.c, big ? -ls : off), LP_FLOOR);
+    const float d = fmaxf(fmaf(x - m, a.c, off), LP_FLOOR);
     const float v = exp2f(d) * fmaf(B, d, A);
     return j == tok ? v + at_token : v;
   };
