@@ -125,3 +125,24 @@ def test_empty_batches():
     assert torch.equal(raw.embedding_grad(none, torch.zeros(2, 0, 4), 3), torch.zeros(3, 4))
     r = raw.token_log_probs(torch.zeros(2, 0, 5), none, 2)
     assert r.log_probs.shape == (2, 0) and r.top_indices.shape == (2, 0, 2)
+
+
+@pytest.mark.parametrize("value,T", [(-1e9, 1.0), (-1e9, 0.1), (-1e10, 0.8), (-1e15, 1.0), (1e10, 0.8), (5000.0, 1e-6), (1e34, 1e-6),
+                                     (torch.finfo(torch.float32).min, 0.8)])
+def test_rows_of_large_logits(value, T):
+    """Rows filled with a finite mask value, large logits, small temperatures: the distances to the maximum count, not the size."""
+    z = torch.full((3, 1000), value)
+    z[1, ::3] = -math.inf
+    z[2, 17:19] = value + abs(value) / 2
+    tokens, g, h = torch.tensor([0, 1, 18]), torch.tensor([0.5, -1.0, 2.0]) * T, torch.tensor([1.0, 0.7, -0.3]) * T
+    lp, ent, tv, ti, *_ = logprobs64(z, tokens, 3, T, -100)
+    z.requires_grad_()
+    r = F.token_log_probs(z, tokens, 3, T)
+    assert torch.equal(r.top_indices, ti)
+    # sums of 1000 equal terms, a logarithm below 7 and a product with it: 1000 steps of 2^-24 each and a few more; the distance to the
+    # maximum, 5e14 among these, its quotient by the temperature, the result and the reference are rounded to fp32 (or are infinite there)
+    for got, ref in ((r.log_probs, lp), (r.entropy, ent), (r.top_log_probs, tv)):
+        assert torch.allclose(got.detach().double(), ref.float().double(), rtol=4 * 2.0 ** -24, atol=7 * 1100 * 2.0 ** -24)
+    (d,) = torch.autograd.grad((r.log_probs, r.entropy), (z,), (g, h))
+    ref, mag = logprobs_grad64(z.detach(), tokens, g, h, T, -100)
+    assert bool(((d.double() - ref).abs() <= 8 * 1100 * 2.0 ** -24 * mag + 1e-12).all())

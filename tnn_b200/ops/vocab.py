@@ -245,13 +245,13 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
 
 def _distribution(z: torch.Tensor, temperature: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``log p``, ``p`` and ``p log p`` of every element, with the conventions of :func:`token_log_probs`."""
-    x = z / temperature
-    m = x.max(1, keepdim=True).values
+    m = z.max(1, keepdim=True).values
     dead = torch.isneginf(m)
     bad = torch.isnan(m) | torch.isposinf(m)
-    m0 = torch.where(dead | bad, torch.zeros_like(m), m)
-    lse = m0 + torch.log(torch.exp(x - m0).sum(1, keepdim=True))
-    logp = torch.where(torch.isneginf(x), x, x - lse)
+    # relative to the maximum before anything is rounded: beside a large one the sum's logarithm would be lost, and a quotient by the
+    # temperature might overflow
+    d = (z - torch.where(dead | bad, torch.zeros_like(m), m)) / temperature
+    logp = torch.where(torch.isneginf(z), z, d - torch.log(torch.exp(d).sum(1, keepdim=True)))
     logp = torch.where(bad, torch.full_like(logp, math.nan), logp)
     p = torch.exp(logp)
     plogp = torch.where(p == 0, torch.zeros_like(p), p * logp)
