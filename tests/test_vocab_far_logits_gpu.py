@@ -83,3 +83,17 @@ def test_the_edge_is_where_it_is_said_to_be():
     for v in (EDGE - 40, EDGE + 40):
         r = raw.token_log_probs(torch.full((1, 77), float(v), device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"))
         assert abs(r.log_probs.item() + math.log(77)) < 1e-5 and abs(r.entropy.item() - math.log(77)) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,weight", [(1e-6, 1e10), (1e-3, 1e16), (0.8, 1e22)])
+def test_large_entropy_gradients_leave_ruled_out_tokens_alone(dtype, T, weight):
+    z = torch.randn(4, 1003, generator=torch.Generator().manual_seed(5)).to(dtype)
+    z[:, 1::2] = -math.inf
+    z[1, 1::2] = torch.finfo(dtype).min
+    z[2, 40:44:2] = 5.0
+    tokens, h = torch.tensor([0, 2, 40, 4], device="cuda"), torch.full((4,), weight, device="cuda")
+    keep = {}
+    raw.token_log_probs(z.cuda(), tokens, 0, T, keep=keep)
+    d = raw.token_log_probs_grad(z.cuda(), tokens, keep, None, h, T)
+    assert bool((d[:, 1::2] == 0).all())

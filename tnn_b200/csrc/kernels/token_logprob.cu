@@ -720,10 +720,10 @@ token_logprob_grad_kernel(const LogprobGradParams a) {
       Logits<T>::pairs(v[u], x);
 #pragma unroll
       for (int j = 0; j < PER / 2; ++j) {
-        const uint64_t d2 = fma_f2(add_f2(x[j], nm2), c2, off2);
         float d0, d1, g0, g1;
-        unpack_f2(d2, d0, d1);
-        unpack_f2(mul_f2(pack_f2(exp2f(d0), exp2f(d1)), fma_f2(B2, d2, A2)), g0, g1);
+        unpack_f2(fma_f2(add_f2(x[j], nm2), c2, off2), d0, d1);
+        d0 = fmaxf(d0, LP_FLOOR), d1 = fmaxf(d1, LP_FLOOR);  // (a product with B must not overflow where the probability is 0)
+        unpack_f2(mul_f2(pack_f2(exp2f(d0), exp2f(d1)), fma_f2(B2, pack_f2(d0, d1), A2)), g0, g1);
         Logits<T>::put(v[u], j, g0, g1);
       }
       T* d = dz + p.head + vi * PER;
