@@ -22,6 +22,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import raw
 from .gemm import gemm
@@ -36,7 +37,7 @@ def _is_plain(t: torch.Tensor) -> bool:
     (``create_graph``), and it is no batch of gradients (``is_grads_batched``, ``vmap``) and no dual number."""
     f = torch._C._functorch
     return not ((t.requires_grad and torch.is_grad_enabled()) or f.is_legacy_batchedtensor(t) or f.is_functorch_wrapped_tensor(t)
-                or torch.autograd.forward_ad._current_level >= 0)
+                or forward_ad._current_level >= 0)
 
 
 def _in_one_launch(rows: int, m: int, n: int) -> bool:
@@ -181,11 +182,22 @@ def cross_entropy(logits: torch.Tensor, labels: torch.Tensor, return_corrects: b
     return (loss, corrects) if return_corrects else loss
 
 
+def _undifferentiated(t: torch.Tensor) -> bool:
+    """Whether no derivative with respect to ``t`` can be asked for, in either mode, so that the operator needs no autograd node: the
+    nodes refuse tangents, a kernel that was called without one would drop them. (The CPU forms are torch operations and carry them.)"""
+    return _is_plain(t) if t.is_cuda else not (t.requires_grad and torch.is_grad_enabled())
+
+
 def _differentiable_once(backward):
-    """``once_differentiable`` where a second derivative may be asked for (``create_graph``): it costs 20 us a call."""
+    """``once_differentiable`` where a second derivative may be asked for (``create_graph``): it costs 20 us a call. A gradient on a GPU
+    that carries a tangent is refused: the kernels see its value alone."""
     guarded = torch.autograd.function.once_differentiable(backward)
 
     def run(ctx, *grads):
+        if forward_ad._current_level >= 0:
+            for g in grads:
+                if g is not None and g.is_cuda and forward_ad.unpack_dual(g).tangent is not None:
+                    raise NotImplementedError("the gradient that enters this operator carries a tangent")
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 
@@ -208,7 +220,7 @@ class _Embedding(torch.autograd.Function):
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * table[ids]`` (zeros at ``padding_idx``), shape ``[*ids.shape, width]``. The table's gradient adds each token's
     positions up in fp32, in an order that depends on the ids alone, and rounds once to the table's type."""
-    if not (table.requires_grad and torch.is_grad_enabled()):
+    if _undifferentiated(table):
         return raw.embedding_lookup(ids, table, scale, padding_idx)
     return _Embedding.apply(ids, table, float(scale), padding_idx)
 
@@ -237,6 +249,6 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
                     ignore_index: int = -100) -> raw.TokenLogProbs:
     """:func:`raw.token_log_probs` with gradients through the log probabilities and the entropies (the alternatives are
     reported, not differentiated): one pass over the logits forward, one read and one write backward."""
-    if not (logits.requires_grad and torch.is_grad_enabled()):
+    if _undifferentiated(logits):
         return raw.token_log_probs(logits, tokens, top_k, temperature, ignore_index)
     return raw.TokenLogProbs(*_TokenLogProbs.apply(logits, tokens, top_k, float(temperature), int(ignore_index)))
