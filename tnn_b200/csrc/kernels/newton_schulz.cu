@@ -778,6 +778,16 @@ static void ns_tiles(NsParams& p) {
   p.x_tiles = p.x_m * p.x_n;
 }
 
+// Which kernel a batch takes: 2 CTA pairs where their tiles keep all of them busy in every product, else 1 with 128 x 128 tiles, for a few
+// tiles 0 with halves of those.
+static int ns_kernel_of(NsParams p) {
+  const int sms = sm_count();
+  ns_tiles<1, 256>(p);
+  if ((long long)p.sym_tiles * p.items >= sms * 2 / 5) return 2;
+  ns_tiles<0, 128>(p);
+  return (long long)p.x_tiles * p.items > sms ? 1 : 0;
+}
+
 template <int PAIR, int BN, int TALL>
 static cudaError_t ns_launch(const NsMaps& maps, NsParams p, cudaStream_t st) {
   using Cfg = NsCfg<PAIR, BN>;
@@ -872,17 +882,19 @@ int tnnb_newton_schulz(const void* g, long long item, long long ld, int type, in
     rc = rc ? rc : ns_map(&maps.add_x[i], p.hi[i], items, m, n, p.ldx, p.item_x, 32);
   }
   if (rc) return rc;
-  // CTA pairs where their tiles keep all of them busy in every product, else 128 x 128 tiles, for a few tiles halves of those.
-  ns_tiles<1, 256>(p);
-  const int sms = sm_count();
-  if ((long long)p.sym_tiles * items >= sms * 2 / 5) {
-    e = tall ? ns_launch<1, 256, 1>(maps, p, st) : ns_launch<1, 256, 0>(maps, p, st);
-  } else {
-    ns_tiles<0, 128>(p);
-    if ((long long)p.x_tiles * items > sms) e = tall ? ns_launch<0, 128, 1>(maps, p, st) : ns_launch<0, 128, 0>(maps, p, st);
-    else e = tall ? ns_launch<0, 64, 1>(maps, p, st) : ns_launch<0, 64, 0>(maps, p, st);
+  switch (ns_kernel_of(p)) {
+    case 2: e = tall ? ns_launch<1, 256, 1>(maps, p, st) : ns_launch<1, 256, 0>(maps, p, st); break;
+    case 1: e = tall ? ns_launch<0, 128, 1>(maps, p, st) : ns_launch<0, 128, 0>(maps, p, st); break;
+    default: e = tall ? ns_launch<0, 64, 1>(maps, p, st) : ns_launch<0, 64, 0>(maps, p, st);
   }
   return e == cudaSuccess ? 0 : -(int)e - 1000;
+}
+
+// Which of its kernels tnnb_newton_schulz takes on the current device (ns_kernel_of).
+int tnnb_newton_schulz_kernel(int items, int m, int n) {
+  NsParams p = {};
+  p.m = m, p.n = n, p.l = m < n ? m : n, p.items = items;
+  return ns_kernel_of(p);
 }
 
 }  // extern "C"
