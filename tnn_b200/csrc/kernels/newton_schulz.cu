@@ -31,6 +31,8 @@
 // product has seen it.
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "gemm_tcgen05.h"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -43,6 +45,7 @@ static constexpr float NS_X = 4096.f, NS_A = 4096.f, NS_B = 2048.f;  // stored =
 static constexpr int NS_EPI_WARPS = 8;
 static constexpr int NS_THREADS = 96 + 32 * NS_EPI_WARPS;
 static constexpr int NS_MAX_STEPS = 64;
+static constexpr int NS_DEVICES = 64;  // whose number of CTA pairs is remembered
 static constexpr int NS_FOLDED = 2;      // last steps in which B holds a
 
 // The parts of a step, in the order in which tiles are dealt out.
@@ -810,14 +813,20 @@ static cudaError_t ns_launch(const NsMaps& maps, NsParams p, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1 + PAIR;
   if (PAIR) {
-    static int pairs = 0;  // that fit at the same time (a group of SMs may have an odd one over)
+    // Pairs that fit at the same time: a group of SMs may have an odd one over, and GPUs of one machine differ in their groups.
+    static std::atomic<int> known[NS_DEVICES];
+    int device = 0;
+    e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    int pairs = device < NS_DEVICES ? known[device].load(std::memory_order_relaxed) : 0;
     if (pairs == 0) {
       cfg.gridDim = dim3(2);
       cfg.attrs = attr + 1, cfg.numAttrs = 1;
-      int n = 0;
-      e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+      e = cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg);
       if (e != cudaSuccess) return e;
-      pairs = n < sms / 2 ? n : sms / 2;
+      pairs = pairs < sms / 2 ? pairs : sms / 2;
+      if (pairs < 1) return cudaErrorCooperativeLaunchTooLarge;
+      if (device < NS_DEVICES) known[device].store(pairs, std::memory_order_relaxed);
       cfg.attrs = attr, cfg.numAttrs = 2;
     }
     cfg.gridDim = dim3((unsigned)(2 * (most < pairs ? most : pairs)));
