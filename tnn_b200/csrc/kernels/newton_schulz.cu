@@ -20,8 +20,11 @@
 // rounded off of the large singular directions would drown the small ones, which grow 480-fold: a matrix of rank one plus noise came
 // out 6 % off (2-norm), with it 0.01 %. What is rounded in front of the last two steps grows 12-fold and 3.4-fold only (0.13 % for that
 // matrix); there a is added to B's diagonal and X <- B X reads nothing beside its operands. Matrices of Gaussian numbers are 0.1 %
-// off, less than the rounding of the result to bf16; the worst of thousands 0.3 % for 32 x 32, 0.5 % for 8 x 8 and 1.6 % for 2 x 2 (the
-// quintic's slope is 3.9 where a singular value has come to 1.2, and the roundings of few elements do not average out).
+// off, less than the rounding of the result to bf16; the worst of thousands 0.3 % for 32 x 32, 0.5 % for 8 x 8 and 1.6 % for 2 x 2: the
+// quintic's slope is 3.9 where a singular value has come to 1.2, and the roundings of few elements do not average out. Nor do those
+// of many equal ones, whatever the size: the identity of 382 rows is 1.2 % off (bf16 result included), a constant matrix of 256 x 768
+// 0.5 %, and of the singular values of [1e-4, 1], one element per row and column, the worst (0.62) 2.7 %. That is the price of operands of 11
+// bits: X with 22 bits in all steps leaves it at 2.7 %, only all products with operands of 22 bits, three times the products, would mend it.
 //
 // Figures (five steps; floor: the products with their symmetry at the measured bf16 rate). 12 x 2304 x 768 fp32 413 - 485 us (167) by the
 // clock that the power limit leaves, 48 of them the two passes of the norm, 8 x 1280 x 5120 bf16 1200 - 1400 (670): a K block of a CTA
