@@ -358,3 +358,17 @@ def test_offsets_beyond_32_bits():
     assert all(torch.equal(x, y) for x, y in zip(a, b))
     g = torch.randn(2, device="cuda")
     assert torch.equal(raw.token_log_probs_grad(rows, one, kept, g, g), raw.token_log_probs_grad(near, one, plain, g, g))
+
+
+@pytest.mark.parametrize("n", [100, 600])
+def test_embedding_gradient_into_the_memory_of_its_input(n):
+    ids = ids_for(n, n, "zipf", 5).cuda()
+    dy = torch.randn(n, 64, device="cuda")
+    ref = raw.embedding_grad(ids, dy, n, 0.5)
+    space = torch.empty(2 * n, 64, device="cuda")
+    for at in (0, 1, n // 2):  # the same rows, and rows some of which are the other's
+        inner = space[at:at + n]
+        inner.copy_(dy)
+        assert torch.equal(raw.embedding_grad(ids, inner, n, 0.5, out=space[:n]), ref)
+    space[:n] = dy
+    assert torch.allclose(raw.embedding_grad(ids, space[:n], n, 0.5, out=space[:n], accumulate=True), ref + dy, atol=1e-6)

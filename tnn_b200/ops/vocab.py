@@ -65,6 +65,12 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     return t if (t.stride(1) == 1 or width == 1) and (t.shape[0] < 2 or t.stride(0) >= width) else t.contiguous()
 
 
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors overlap."""
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def _new(like: torch.Tensor, dtype, *sizes: int) -> torch.Tensor:
     return torch.empty(sizes, dtype=dtype, device=like.device)  # (_lib.empty takes eight dimensions)
 
@@ -146,6 +152,8 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
         with _lib.device_of(dy2):
             if out is None:
                 out = _lib.empty(dy2, rows, width)
+            elif n and _share_memory(out, dy2):
+                dy2 = dy2.clone(memory_format=torch.contiguous_format)  # rows are written while others are still read
             pitch = max(_pitch(dy2), width) if n else width
             if n <= _FEW:
                 rc = _library().tnnb_embed_grad(flat, flat.dtype is torch.int64, dy2, pitch, out, None, None, None, None, None, n, width, rows, pad,
