@@ -146,3 +146,13 @@ def test_rows_of_large_logits(value, T):
     (d,) = torch.autograd.grad((r.log_probs, r.entropy), (z,), (g, h))
     ref, mag = logprobs_grad64(z.detach(), tokens, g, h, T, -100)
     assert bool(((d.double() - ref).abs() <= 8 * 1100 * 2.0 ** -24 * mag + 1e-12).all())
+
+
+def test_rows_longer_than_32_bit_counts_are_refused():
+    """Widths beyond 32 bits were cut off on their way into the kernels."""
+    ids, one = torch.zeros(1, dtype=torch.int64), torch.zeros(1, 1)
+    for width in (2 ** 30 + 1, 2 ** 31 + 8, 2 ** 32 + 8):
+        with pytest.raises(ValueError):
+            raw.embedding_lookup(ids, one.expand(1, width))
+        with pytest.raises(ValueError):
+            raw.embedding_grad(ids, one.expand(1, width), 1)

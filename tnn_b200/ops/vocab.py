@@ -17,6 +17,7 @@ from .gemm import LAUNCHES
 MAX_TOP = 32  # alternatives per row
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _NO_PADDING = -(1 << 63)  # an id that no table has
+_MAX_WIDTH = 1 << 30  # columns of a table: the kernels count them in 32 bits
 _LOG2E = 1.4426950408889634
 _DECLARED = False
 
@@ -90,6 +91,8 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     n = flat.numel()
     if n and (rows == 0 or width == 0):
         raise ValueError(f"embedding table {tuple(table.shape)} is empty")
+    if width > _MAX_WIDTH:
+        raise ValueError(f"rows of {width} elements: at most {_MAX_WIDTH} are supported")
     pad = _NO_PADDING if padding_idx is None else int(padding_idx)
     if table.is_cuda:
         code = _type_code(table, "embedding table")
@@ -136,8 +139,8 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
         raise ValueError(f"the gradient of a table of {rows} rows of {width} elements is empty")
     flat = _whole(ids, dy, "ids")
     n = flat.numel()
-    if n >= 1 << 30 or rows > 1 << 24:
-        raise ValueError(f"{n} positions and {rows} rows: fewer than 2^30 and at most 2^24 are supported")
+    if n >= 1 << 30 or rows > 1 << 24 or width > _MAX_WIDTH:
+        raise ValueError(f"{n} positions, {rows} rows of {width} elements: fewer than 2^30, at most 2^24 of at most {_MAX_WIDTH} are supported")
     if accumulate and out is None:
         raise ValueError("accumulate needs an output to add to")
     if out is not None:
