@@ -264,3 +264,35 @@ def test_replicas_reduced_by_the_library():
         one.update()
         two.update()
     assert torch.equal(g1.master_flat, g2.master_flat)
+
+
+BAD_PIECES = [(60, 5, 0), (-1, 3, 0), (0, 3, 18), (5, 4, -2), (5, -4, 2), (2 ** 62, 2 ** 62, 0), (0, 2 ** 63 - 1, 2 ** 63 - 1)]
+
+
+@pytest.mark.parametrize("bad", BAD_PIECES)
+def test_pieces_outside_of_the_buffers_on_the_cpu(bad):
+    w = torch.ones(64)
+    m, v = torch.zeros(20), torch.zeros(20)
+    with pytest.raises(ValueError):
+        raw.adam_pieces(w, None, torch.ones(64), m, v, torch.tensor([(3, 4, 0), bad]), 0.1, 0.9, 0.95, 1e-8, 0.0, 1)
+    assert torch.equal(w, torch.ones(64)) and not bool(m.any())
+
+
+@gpu
+@pytest.mark.parametrize("bad", BAD_PIECES)
+def test_pieces_outside_of_the_buffers_on_the_gpu(bad):
+    """Left out and recorded; the others are worked on."""
+    from tnn_b200.ops import _lib
+
+    w, ref, grads = (torch.ones(64, device="cuda") for _ in range(3))
+    state, state_ref = torch.zeros(2, 20, device="cuda"), torch.zeros(2, 20, device="cuda")
+    good = torch.tensor([(3, 4, 0), (48, 16, 4)], device="cuda")
+    both = torch.cat([good[:1], torch.tensor([bad], device="cuda"), good[1:]])
+    _lib.check_status()
+    raw.adam_pieces(ref, None, grads, *state_ref, good, 0.1, 0.9, 0.95, 1e-8, 0.0, 1)
+    _lib.check_status()
+    raw.adam_pieces(w, None, grads, *state, both, 0.1, 0.9, 0.95, 1e-8, 0.0, 1)
+    with pytest.raises(RuntimeError):
+        _lib.check_status()
+    assert torch.equal(w, ref) and torch.equal(state, state_ref)
+    _lib.check_status()

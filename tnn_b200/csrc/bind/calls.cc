@@ -76,7 +76,7 @@ const Entry SIGNATURES[] = {
     SIG("piplplillfip"), SIG("piplpppppp" "iillfiiiip"),  // embed_lookup, embed_grad
     SIG("plpipppppliiflip"), SIG("plplpipppp" "liffl" "ip"),  // token_logprob, token_logprob_grad
     SIG("plliiiipif" "pppppppppp"),  // newton_schulz
-    SIG("ppppilfifpip"), SIG("ppppil" "fffpip"), SIG("ppppppi" "fffffffffpp"),  // muon_momentum, muon_apply, adam_pieces
+    SIG("ppppilfifpip"), SIG("ppppil" "fffpip"), SIG("ppppppill" "fffffffffppp"),  // muon_momentum, muon_apply, adam_pieces
     SIG("plplip"), SIG("pplp"), SIG("plpplip"),         // colsum_accum, cast_f32_bf16, scale_by
     SIG("pppppppp" "liffupp"),                          // layernorm_fwd
     SIG("pppppppppp" "lifupp"), SIG("ppppppppppp" "lifupp"),  // layernorm_bwd, layernorm_bwd_db

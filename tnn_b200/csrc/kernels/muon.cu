@@ -59,15 +59,20 @@ muon_apply_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ low, c
   }
 }
 
-// Adam (the formula of loss_optim.cu) over pieces of the flat buffers: a block takes piece {offset, length, place of its state}.
+// Adam (the formula of loss_optim.cu) over pieces of the flat buffers: a block takes piece {offset, length, place of its state}. One that
+// does not lie in the buffers (`total` elements, `states` of state) is left out and recorded.
 __global__ void __launch_bounds__(256)
 adam_pieces_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ low, const float* __restrict__ grads, float* __restrict__ m,
-                   float* __restrict__ v, const long long* __restrict__ pieces, float lr, float b1, float b2, float eps, float wd,
-                   float bc1, float bc2, float gscale, float lr_ratio, const float* __restrict__ hyper) {
+                   float* __restrict__ v, const long long* __restrict__ pieces, long long total, long long states, float lr, float b1, float b2,
+                   float eps, float wd, float bc1, float bc2, float gscale, float lr_ratio, const float* __restrict__ hyper, int* status) {
   if (hyper) lr = hyper[0], bc1 = hyper[1], bc2 = hyper[2], gscale = hyper[3];
   lr *= lr_ratio;
   const long long* p = pieces + 3ll * blockIdx.x;
   const long long at = p[0], n = p[1], st = p[2];
+  if (at < 0 || st < 0 || n < 0 || n > total || n > states || at > total - n || st > states - n) {
+    if (threadIdx.x == 0 && status) atomicCAS(status, 0, ST_BAD_ARG);
+    return;
+  }
   const float ib1 = 1.f / bc1, ib2 = 1.f / bc2;
   for (long long i = threadIdx.x; i < n; i += 256) {
     const float g = grads[at + i] * gscale;
@@ -116,14 +121,15 @@ int tnnb_muon_apply(void* master, void* low, const void* offsets, const void* up
   return e == cudaSuccess ? 0 : -(int)e - 1000;
 }
 
-// pieces: int64 [count][3] on the device: offset in the flat buffers, length, place in m and v.
-int tnnb_adam_pieces(void* master, void* low, const void* grads, void* m, void* v, const void* pieces, int count, float lr, float b1, float b2,
-                     float eps, float wd, float bc1, float bc2, float gscale, float lr_ratio, const void* hyper, void* stream) {
-  if (count < 0) return -3;
+// pieces: int64 [count][3] on the device: offset in the flat buffers (`total` elements), length, place in m and v (`states`).
+int tnnb_adam_pieces(void* master, void* low, const void* grads, void* m, void* v, const void* pieces, int count, long long total,
+                     long long states, float lr, float b1, float b2, float eps, float wd, float bc1, float bc2, float gscale, float lr_ratio,
+                     const void* hyper, int* status, void* stream) {
+  if (count < 0 || total < 0 || states < 0) return -3;
   if (count == 0) return 0;
   adam_pieces_kernel<<<count, 256, 0, (cudaStream_t)stream>>>((float*)master, (__nv_bfloat16*)low, (const float*)grads, (float*)m, (float*)v,
-                                                             (const long long*)pieces, lr, b1, b2, eps, wd, bc1, bc2, gscale, lr_ratio,
-                                                             (const float*)hyper);
+                                                             (const long long*)pieces, total, states, lr, b1, b2, eps, wd, bc1, bc2, gscale,
+                                                             lr_ratio, (const float*)hyper, status);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e - 1000;
 }

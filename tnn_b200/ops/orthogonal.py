@@ -142,7 +142,7 @@ def _muon_library():
         p, i, l, f = _lib.c_void_p, _lib.c_int, _lib.c_ll, _lib.c_float
         _lib.declare(lib, "tnnb_muon_momentum", [p, p, p, p, i, l, f, i, f, p, i, p])
         _lib.declare(lib, "tnnb_muon_apply", [p, p, p, p, i, l, f, f, f, p, i, p])
-        _lib.declare(lib, "tnnb_adam_pieces", [p, p, p, p, p, p, i, f, f, f, f, f, f, f, f, f, p, p])
+        _lib.declare(lib, "tnnb_adam_pieces", [p, p, p, p, p, p, i, l, l, f, f, f, f, f, f, f, f, f, p, p, p])
         _MUON_DECLARED = True
     return lib
 
@@ -227,7 +227,8 @@ def muon_apply(master: torch.Tensor, low, group: MatrixGroup, update: torch.Tens
 def adam_pieces(master: torch.Tensor, low, grads: torch.Tensor, m: torch.Tensor, v: torch.Tensor, pieces: torch.Tensor, lr: float, b1: float,
                 b2: float, eps: float, wd: float, step: int, gscale: float = 1.0, lr_ratio: float = 1.0, hyper=None) -> None:
     """:func:`raw.adam_step` over pieces of the flat buffers: ``pieces`` int64 ``[count, 3]``, on the buffers' device: offset, length and
-    place in the packed moments ``m``, ``v``; no element in two pieces."""
+    place in the packed moments ``m``, ``v``; no element in two pieces. A piece that does not lie in the buffers raises ``ValueError`` on CPU; on
+    CUDA it is left out and recorded (``_lib.check_status``)."""
     for t, what in ((master, "weights"), (grads, "gradients"), (m, "moments"), (v, "moments")):
         if t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous() or t.device != master.device:
             raise ValueError(f"{what} {tuple(t.shape)} of {t.dtype} on {t.device}: packed fp32 on {master.device} expected")
@@ -239,15 +240,19 @@ def adam_pieces(master: torch.Tensor, low, grads: torch.Tensor, m: torch.Tensor,
     bc1, bc2 = 1 - b1 ** step, 1 - b2 ** step
     if master.is_cuda:
         with _lib.device_of(master):
-            rc = _muon_library().tnnb_adam_pieces(master, low, grads, m, v, pieces, pieces.shape[0], lr, b1, b2, eps, wd, bc1, bc2, gscale, lr_ratio,
-                                                  hyper, _lib.raw_stream())
+            rc = _muon_library().tnnb_adam_pieces(master, low, grads, m, v, pieces, pieces.shape[0], master.numel(), m.numel(), lr, b1, b2, eps, wd,
+                                                  bc1, bc2, gscale, lr_ratio, hyper, _lib.status_addr(master.device), _lib.raw_stream())
             _lib.check_rc(rc, "adam_pieces")
             LAUNCHES["count"] += 1
         return
     if hyper is not None:
         lr, bc1, bc2, gscale = (float(x) for x in hyper)
     rate = lr * lr_ratio
-    for at, n, st in pieces.tolist():
+    places = pieces.tolist()
+    for at, n, st in places:
+        if min(at, n, st) < 0 or at + n > master.numel() or st + n > m.numel():
+            raise ValueError(f"a piece of {n} elements at {at}, its state at {st}: {master.numel()} weights, {m.numel()} moments")
+    for at, n, st in places:
         g = grads[at:at + n].float() * gscale
         mi, vi, w = m[st:st + n], v[st:st + n], master[at:at + n]
         mi.mul_(b1).add_(g, alpha=1 - b1)
