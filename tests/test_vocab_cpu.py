@@ -156,3 +156,22 @@ def test_rows_longer_than_32_bit_counts_are_refused():
             raw.embedding_lookup(ids, one.expand(1, width))
         with pytest.raises(ValueError):
             raw.embedding_grad(ids, one.expand(1, width), 1)
+
+
+IDS_OF_NOTHING = [None, 2 ** 64, -2 ** 64 + 3, 2 ** 63, 2 ** 32, 2 ** 31 + 1]
+
+
+@pytest.mark.parametrize("value", IDS_OF_NOTHING)
+def test_ids_that_no_tensor_holds(value, dev="cpu"):
+    """A padding index or an ignored token beyond 32 or 64 bits is no id's, whatever its lowest bits are."""
+    ids, table = torch.tensor([0, 1, 3, -1], device=dev), torch.randn(5, 8, device=dev)
+    z, tokens = torch.randn(4, 9, device=dev), torch.tensor([0, 1, 3, 2], device=dev)
+    far = -7 if value is None else value
+    for kind in (torch.int64, torch.int32):
+        assert torch.equal(raw.embedding_lookup(ids.to(kind), table, 1.0, value), raw.embedding_lookup(ids, table))
+        assert torch.equal(raw.embedding_grad(ids.to(kind), table[:4], 5, 1.0, value), raw.embedding_grad(ids, table[:4], 5))
+        kept, plain = {}, {}
+        for a, b in zip(raw.token_log_probs(z, tokens.to(kind), 2, 1.0, far, kept), raw.token_log_probs(z, tokens, 2, keep=plain)):
+            assert torch.equal(a, b)
+        assert torch.equal(raw.token_log_probs_grad(z, tokens.to(kind), kept, z[:, 0], z[:, 1], 1.0, far),
+                           raw.token_log_probs_grad(z, tokens, plain, z[:, 0], z[:, 1]))

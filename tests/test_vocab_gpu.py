@@ -372,3 +372,10 @@ def test_embedding_gradient_into_the_memory_of_its_input(n):
         assert torch.equal(raw.embedding_grad(ids, inner, n, 0.5, out=space[:n]), ref)
     space[:n] = dy
     assert torch.allclose(raw.embedding_grad(ids, space[:n], n, 0.5, out=space[:n], accumulate=True), ref + dy, atol=1e-6)
+
+
+def test_ids_that_no_tensor_holds():
+    from tests.test_vocab_cpu import IDS_OF_NOTHING, test_ids_that_no_tensor_holds as check
+
+    for value in IDS_OF_NOTHING:
+        check(value, "cuda")

@@ -16,7 +16,7 @@ from .gemm import LAUNCHES
 
 MAX_TOP = 32  # alternatives per row
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_NO_PADDING = -(1 << 63)  # an id that no table has
+_NO_ID = -(1 << 63)  # an id that no table has
 _MAX_WIDTH = 1 << 30  # columns of a table: the kernels count them in 32 bits
 _LOG2E = 1.4426950408889634
 _DECLARED = False
@@ -57,6 +57,11 @@ def _whole(t: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _id(value: Optional[int]) -> int:
+    """A padding index or ignored token as the kernels compare it: one beyond 64 bits, like None, is no id's."""
+    return _NO_ID if value is None or not _NO_ID < int(value) < -_NO_ID else int(value)
+
+
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """``[rows, width]`` with a unit inner stride and rows that do not overlap."""
     if t.dim() != 2:
@@ -93,7 +98,7 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         raise ValueError(f"embedding table {tuple(table.shape)} is empty")
     if width > _MAX_WIDTH:
         raise ValueError(f"rows of {width} elements: at most {_MAX_WIDTH} are supported")
-    pad = _NO_PADDING if padding_idx is None else int(padding_idx)
+    pad = _id(padding_idx)
     if table.is_cuda:
         code = _type_code(table, "embedding table")
         table = _rows(table, width)
@@ -105,8 +110,8 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
                 _lib.check_rc(rc, "embedding_lookup")
                 LAUNCHES["count"] += 1
         return out
-    flat = flat.reshape(-1)
-    safe = torch.where((flat < 0) | (flat >= rows), torch.zeros_like(flat), flat).long()
+    flat = flat.reshape(-1).long()  # (compared as 32 bits, an index beyond them is cut off: no padding index was id 0)
+    safe = torch.where((flat < 0) | (flat >= rows), torch.zeros_like(flat), flat)
     wide = torch.promote_types(table.dtype, torch.float32)
     out = table[safe].to(wide) * scale
     out = torch.where((flat == pad)[:, None], torch.zeros_like(out), out)
@@ -148,7 +153,7 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
             raise ValueError(f"out {tuple(out.shape)} on {out.device}: a packed [{rows}, {width}] on {dy.device} expected")
         if out.dtype not in ((torch.float32,) if accumulate else (dy.dtype, torch.float32)):
             raise TypeError(f"out is {out.dtype} for gradients of {dy.dtype}" + (" that are added up in fp32" if accumulate else ""))
-    pad = _NO_PADDING if padding_idx is None else int(padding_idx)
+    pad = _id(padding_idx)
     if dy.is_cuda:
         code = _type_code(dy, "dy")
         dy2 = _rows(dy, width)
@@ -176,8 +181,8 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
             _lib.check_rc(rc, "embedding_grad")
             LAUNCHES["count"] += 4
         return out
-    flat = flat.reshape(-1)
-    safe = torch.where((flat < 0) | (flat >= rows), torch.zeros_like(flat), flat).long()
+    flat = flat.reshape(-1).long()  # (compared as 32 bits, an index beyond them is cut off: no padding index was id 0)
+    safe = torch.where((flat < 0) | (flat >= rows), torch.zeros_like(flat), flat)
     g = dy.reshape(-1, width).to(torch.promote_types(dy.dtype, torch.float32))
     g = torch.where((flat == pad)[:, None], torch.zeros_like(g), g)
     total = torch.zeros(rows, width, dtype=g.dtype).index_add_(0, safe, g) * scale
@@ -217,7 +222,7 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
     the vocabulary has log probability NaN. A row with nothing but -inf has log probability -inf and entropy 0; a NaN or +inf logit
     makes a row's results NaN (NaN sorts first, and the indices are those of the largest logits all the same). ``keep``: a dict that
     receives what :func:`token_log_probs_grad` needs."""
-    top_k, temperature, shape = int(top_k), float(temperature), tokens.shape
+    top_k, temperature, ignore_index, shape = int(top_k), float(temperature), _id(ignore_index), tokens.shape
     V = _check_rows(logits, tokens, top_k, temperature)
     tok = _whole(tokens, logits, "tokens")
     z = _rows(logits, V)
@@ -232,18 +237,18 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
             stats = _lib.empty(z, f32, rows, 2) if keep is not None else None
             if rows:
                 rc = _library().tnnb_token_logprob(z.data_ptr(), max(_pitch(z), V), tok, tok.dtype is torch.int64, lp, ent, top, idx, stats, rows, V, top_k,
-                                                   _LOG2E / temperature, int(ignore_index), code, _lib.raw_stream())
+                                                   _LOG2E / temperature, ignore_index, code, _lib.raw_stream())
                 _lib.check_rc(rc, "token_log_probs")
                 LAUNCHES["count"] += 1
         if keep is not None:
             keep.update(stats=stats, entropy=ent)
         return TokenLogProbs(lp, ent, top, idx)
-    tok = tok.reshape(-1)
+    tok = tok.reshape(-1).long()
     wide = torch.promote_types(z.dtype, torch.float32)
     zf = z.to(wide)
     logp, p, plogp = _distribution(zf, temperature)
     known = (tok >= 0) & (tok < V)
-    lp = logp.gather(1, torch.where(known, tok, torch.zeros_like(tok)).long()[:, None])[:, 0]
+    lp = logp.gather(1, torch.where(known, tok, torch.zeros_like(tok))[:, None])[:, 0]
     lp = torch.where(known, lp, torch.full_like(lp, math.nan))
     lp = torch.where(tok == ignore_index, torch.zeros_like(lp), lp)
     # explicit keys: torch orders -0 and 0 as equal, NaN above everything, which is the order wanted
@@ -279,6 +284,7 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
     forward call left in its ``keep``. Rows without a distribution get zeros. The result has the shape of ``logits`` and, where the
     gaps between its rows are smaller than a row, the same gaps."""
     V = _check_rows(logits, tokens, 0, float(temperature))
+    ignore_index = _id(ignore_index)
     tok = _whole(tokens, logits, "tokens")
     z = _rows(logits, V)
     rows = z.shape[0]
@@ -309,13 +315,13 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
             if rows:
                 rc = _library().tnnb_token_logprob_grad(z.data_ptr(), pitch, dz, out_pitch, tok, tok.dtype is torch.int64, stats, entropy,
                                                         g, h, rows, V, _LOG2E / float(temperature), 1.0 / float(temperature),
-                                                        int(ignore_index), code, _lib.raw_stream())
+                                                        ignore_index, code, _lib.raw_stream())
                 _lib.check_rc(rc, "token_log_probs_grad")
                 LAUNCHES["count"] += 1
         if logits.dim() == 2:
             return dz
         return dz.view(logits.shape) if out_pitch == V else dz.unflatten(0, logits.shape[:-1])
-    tok = tok.reshape(-1)
+    tok = tok.reshape(-1).long()
     zf = z.to(torch.promote_types(z.dtype, torch.float32))
     logp, p, plogp = _distribution(zf, float(temperature))
     dead = torch.isneginf(zf).all(1)
@@ -326,5 +332,5 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
     known = (tok >= 0) & (tok < V)
     g = torch.where((tok != ignore_index) & ~known, torch.full_like(g, math.nan), g)
     d = -p * g[:, None] - h[:, None] * (plogp + p * kept["entropy"].reshape(-1, 1))
-    d.scatter_add_(1, torch.where(known, tok, torch.zeros_like(tok)).long()[:, None], torch.where(known, g, nothing)[:, None])
+    d.scatter_add_(1, torch.where(known, tok, torch.zeros_like(tok))[:, None], torch.where(known, g, nothing)[:, None])
     return torch.where(dead[:, None], torch.zeros_like(d), d / float(temperature)).to(logits.dtype).view(logits.shape)
