@@ -184,8 +184,9 @@ def cross_entropy(logits: torch.Tensor, labels: torch.Tensor, return_corrects: b
 
 def _undifferentiated(t: torch.Tensor) -> bool:
     """Whether no derivative with respect to ``t`` can be asked for, in either mode, so that the operator needs no autograd node: the
-    nodes refuse tangents, a kernel that was called without one would drop them. (The CPU forms are torch operations and carry them.)"""
-    return _is_plain(t) if t.is_cuda else not (t.requires_grad and torch.is_grad_enabled())
+    nodes refuse tangents, a kernel that was called without one would drop them. (The CPU forms are torch operations and carry them;
+    tensors of ``torch.func`` have no memory that a kernel could be given, and are refused with or without a node.)"""
+    return not (t.requires_grad and torch.is_grad_enabled()) and (forward_ad._current_level < 0 or not t.is_cuda)
 
 
 def _differentiable_once(backward):

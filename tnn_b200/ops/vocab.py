@@ -57,9 +57,10 @@ def _whole(t: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _id(value: Optional[int]) -> int:
-    """A padding index or ignored token as the kernels compare it: one beyond 64 bits, like None, is no id's."""
-    return _NO_ID if value is None or not _NO_ID < int(value) < -_NO_ID else int(value)
+def _id(value: int) -> int:
+    """A padding index or ignored token as the kernels compare it: one beyond 64 bits is no id's."""
+    value = int(value)
+    return value if _NO_ID < value < -_NO_ID else _NO_ID
 
 
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
@@ -98,7 +99,7 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         raise ValueError(f"embedding table {tuple(table.shape)} is empty")
     if width > _MAX_WIDTH:
         raise ValueError(f"rows of {width} elements: at most {_MAX_WIDTH} are supported")
-    pad = _id(padding_idx)
+    pad = _NO_ID if padding_idx is None else _id(padding_idx)
     if table.is_cuda:
         code = _type_code(table, "embedding table")
         table = _rows(table, width)
@@ -153,7 +154,7 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, rows: int, scale: float 
             raise ValueError(f"out {tuple(out.shape)} on {out.device}: a packed [{rows}, {width}] on {dy.device} expected")
         if out.dtype not in ((torch.float32,) if accumulate else (dy.dtype, torch.float32)):
             raise TypeError(f"out is {out.dtype} for gradients of {dy.dtype}" + (" that are added up in fp32" if accumulate else ""))
-    pad = _id(padding_idx)
+    pad = _NO_ID if padding_idx is None else _id(padding_idx)
     if dy.is_cuda:
         code = _type_code(dy, "dy")
         dy2 = _rows(dy, width)
