@@ -175,3 +175,12 @@ def test_ids_that_no_tensor_holds(value, dev="cpu"):
             assert torch.equal(a, b)
         assert torch.equal(raw.token_log_probs_grad(z, tokens.to(kind), kept, z[:, 0], z[:, 1], 1.0, far),
                            raw.token_log_probs_grad(z, tokens, plain, z[:, 0], z[:, 1]))
+
+
+def test_kept_entropies_of_other_rows_are_refused():
+    """One row's would be spread over all of them."""
+    z, tokens, g, keep = torch.randn(4, 30), torch.zeros(4, dtype=torch.int64), torch.ones(4), {}
+    raw.token_log_probs(z[:1], tokens[:1], keep=keep)
+    for bad in (keep, {"stats": None, "entropy": torch.zeros(3)}, {"stats": None, "entropy": None}):
+        with pytest.raises(ValueError):
+            raw.token_log_probs_grad(z, tokens, bad, None, g)

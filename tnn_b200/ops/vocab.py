@@ -322,6 +322,9 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
         if logits.dim() == 2:
             return dz
         return dz.view(logits.shape) if out_pitch == V else dz.unflatten(0, logits.shape[:-1])
+    entropy = kept["entropy"]
+    if entropy is None or entropy.numel() != rows or entropy.device != z.device:
+        raise ValueError(f"the entropies that were kept do not belong to {rows} rows on {z.device}")
     tok = tok.reshape(-1).long()
     zf = z.to(torch.promote_types(z.dtype, torch.float32))
     logp, p, plogp = _distribution(zf, float(temperature))
@@ -332,6 +335,6 @@ def token_log_probs_grad(logits: torch.Tensor, tokens: torch.Tensor, kept: dict,
     h = torch.where(dead, nothing, h) if h is not None else nothing
     known = (tok >= 0) & (tok < V)
     g = torch.where((tok != ignore_index) & ~known, torch.full_like(g, math.nan), g)
-    d = -p * g[:, None] - h[:, None] * (plogp + p * kept["entropy"].reshape(-1, 1))
+    d = -p * g[:, None] - h[:, None] * (plogp + p * entropy.reshape(-1, 1))
     d.scatter_add_(1, torch.where(known, tok, torch.zeros_like(tok))[:, None], torch.where(known, g, nothing)[:, None])
     return torch.where(dead[:, None], torch.zeros_like(d), d / float(temperature)).to(logits.dtype).view(logits.shape)
