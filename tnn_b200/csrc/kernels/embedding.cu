@@ -7,7 +7,8 @@
 // (and adds to) row 0 like the layers' embedding kernels (elementwise.cu); the bounds-checked build records it.
 //
 // The gradient adds up in an order that depends on the ids alone: the positions of each token as sorted, in chunks of the sorted list,
-// then the chunks. No atomics on values: the same inputs give the same bits, and a row is written once, in the table's own type.
+// then the chunks: the same inputs give the same bits. A row is written once, in the table's own type; sums that are added to a gradient are
+// added by the memory, each element by one thread, or by one after the kernel of the others has ended.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "values.cuh"
@@ -67,6 +68,10 @@ embed_lookup_kernel(const ID* __restrict__ ids, const T* __restrict__ table, lon
 // with ranges of rows the CTA that had them took 16 us for 8192 tokens of text, 63 for 50001. The list is in this order of rows
 // ("slots"), which is as good as any. Looking twice at every position cost 17 us of 97 for 50001 positions
 // of 1001 fp32 columns.
+//
+// Up to 65536 rows there are 128 CTAs, beyond that one per 512 rows, each of which reads all ids: the work grows with positions times
+// rows. Sums added to a gradient of 16 columns (nothing is cleared then), 8192 and 65536 positions: 65536 rows 22 and 34 us, 2^18 rows 30
+// and 56, 2^20 71 and 127, 2^24 0.9 and 1.5 ms. Clearing the rows that nobody names is dearer there: 2^24 rows of 32 bytes 7.7 ms.
 static constexpr int SORT_WARPS = 32;
 static constexpr int SORT_ROWS = 512;  // most rows of a CTA, one per thread
 static constexpr int SORT_NOTES = 512;  // most positions that a warp notes: row in 9 bits, place in its stretch in 23
@@ -86,8 +91,9 @@ __host__ __device__ __forceinline__ Slots slots_of(long long vocab) {
 __host__ __device__ __forceinline__ int sort_stretch(int n) { return (int)(((n + SORT_WARPS - 1ll) / SORT_WARPS + 127) / 128 * 128); }  // positions of a warp
 __device__ __forceinline__ int slot_of(const Slots& s, int row) { return (row & ((1 << s.bits) - 1)) * s.rows + (row >> s.bits); }
 
-// A position's CTA and the row's number there, 16 bits each (NO_CODE: padding). Every CTA looks at every position twice: what it
-// does to an id is done once, here, and four instructions are left (200000 positions: 28 us per look with the ids themselves).
+// A position's CTA and the row's number there, 16 bits each (NO_CODE: padding). Every CTA looks at every position, and warps with more of
+// their own than they can note do so twice: what can be done to an id once is done here, and four instructions are left (200000 positions:
+// 28 us per look with the ids themselves).
 static constexpr uint32_t NO_CODE = 0xffffffffu;
 template <typename ID>
 __global__ void __launch_bounds__(256)

@@ -27,9 +27,10 @@
 // bits: X with 22 bits in all steps leaves it at 2.7 %, only all products with operands of 22 bits, three times the products, would mend it.
 //
 // Figures (five steps; floor: the products with their symmetry at the measured bf16 rate). 12 x 2304 x 768 fp32 413 - 485 us (167) by the
-// clock that the power limit leaves, 48 of them the two passes of the norm, 8 x 1280 x 5120 bf16 1200 - 1400 (670): a K block of a CTA
-// pair takes 0.38 to 0.46 us, the rate of the library's products, the rest is what no tile overlaps (a product's last round, epilogues
-// with two addends). One 768 x 768 matrix 124 us (6), 9 x 321 x 1155 168 (11): fifteen products in a row, each 1 us to the first
+// clock that the power limit leaves: about 60 in front of the products (the two passes of the norm are 48), 61 for each of the last two
+// steps, 74 to 78 for one whose epilogue has two addends. The library's fp16 products of these shapes, with half of the symmetric ones,
+// take 51 a step. 8 x 1280 x 5120 bf16 1140 - 1400 (670): about 90 in front, 186 to 230 a step, the library's products 195; a K block of a CTA
+// pair takes 0.38 to 0.46 us. One 768 x 768 matrix 124 us (6), 9 x 321 x 1155 168 (11): fifteen products in a row, each 1 us to the first
 // copy, 0.3 us per K block (what one SM gets out of L2, 80 GB/s), 0.6 to 1.6 us of epilogue and 1.9 us until the next
 // product has seen it.
 #include <cuda_fp16.h>
@@ -785,7 +786,11 @@ static void ns_tiles(NsParams& p) {
 }
 
 // Which kernel a batch takes: 2 CTA pairs where their tiles keep all of them busy in every product, else 1 with 128 x 128 tiles, for a few
-// tiles 0 with halves of those.
+// tiles 0 with halves of those. Us of the kernels 0, 1 and 2 (the one taken is marked): 768 x 768, 1 matrix 128*, 154, 206, 4 153*, 162, 210, 6 190, 175*,
+// 215, 9 267, 200*, 239, 10 294, 210, 241*, 16 462, 303, 269*; 2304 x 768, 2 of them 217, 219*, 245, 4 334, 275*, 272, 8 569, 414*, 328, 12 867, 555, 405*; 256 x
+// 512, 20 112, 124*, 139, 40 171, 150*, 166, 64 225, 173, 171*, 120 399, 286, 246*; 321 x 1155, 5 139, 155*, 173, 9 178, 169*, 190, 18 307, 237*, 235, 24 361, 285,
+// 276*; 1280 x 5120, 1 493, 457*, 419, 3 1164, 765*, 536, 5 2058, 1179, 801*. Matrices that are much longer than wide would take pairs
+// from half as many tiles on (up to 43 % in these), and matrices of one tile never (300 of 128 x 128: 163, 124, 271*).
 static int ns_kernel_of(NsParams p) {
   const int sms = sm_count();
   ns_tiles<1, 256>(p);

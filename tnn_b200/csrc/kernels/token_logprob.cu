@@ -244,7 +244,7 @@ struct LogprobShared {
   };
   alignas(16) uint32_t group[LP_GROUPS];
   uint32_t bound;
-  int winners, found, total;
+  int winners, found;
   int winner[NT];
   int warp_count[NT / 32];
   Sums part[NT / 32];
@@ -252,11 +252,10 @@ struct LogprobShared {
   unsigned long long best[LP_TOP];  // this CTA's, in order; 0 past the last
 };
 
-// A row's part: elements [head_lo, head_hi) and [tail_lo, tail_hi) one by one, vectors [v_lo, v_hi) between (vector v begins at
-// element head + v * PER).
+// A row's part: its elements [lo, hi) are the vectors [v_lo, v_hi) (vector v begins at element head + v * PER) and what lies outside of
+// vectors (`loose`): the row's first `head` elements in the first part, those behind the last vector in the last.
 struct RowPart {
-  int head, v_lo, v_hi, lo, hi;  // lo, hi: the part's elements
-  int singles_lo, singles_n;     // elements outside of vectors: the head in the first part, the tail in the last
+  int head, v_lo, v_hi, lo, hi;
 };
 
 template <typename T>
@@ -746,8 +745,10 @@ int tnnb_token_logprob(const void* z, long long ld, const void* tokens, int toke
   if (rows < 0 || V <= 0 || top < 0 || top > LP_TOP || top > V || (rows > 1 && ld < V)) return -3;
   if (rows * LP_CLUSTER > 0x7fffffffLL) return -3;
   if (rows == 0) return 0;
-  // A CTA gets about 18 KB per us out of memory when it is alone on its SM; a cluster costs 2 us. Us with 1, 2, 4 and 8 CTAs per row:
-  // 8 x 50257 bf16 11.3, 10.6, 9.5, 10.1; 8 x 128001 fp32 19.9, 14.4, 11.2, 9.5; 20 x 20000 bf16 7.0, 8.1, 8.3, 8.5; 148 x 50257 9.7, 10.8, 13.8, 20.8.
+  // A CTA gets about 18 KB per us out of memory when it is alone on its SM; a cluster costs 2 us. Us with 1, 2, 4 and 8 CTAs per row, without
+  // alternatives (one call after the other: 8 x 50257 bf16 11.3, 10.6, 9.5, 10.1; 8 x 128001 fp32 19.9, 14.4, 11.2, 9.5; 20 x 20000 bf16 7.0, 8.1, 8.3, 8.5;
+  // 148 x 50257 9.7, 10.8, 13.8, 20.8) and with 20 of them (graph replays, whose times come in steps of 2: 12.4 each; 22.6, 18.6, 14.5, 14.5; 10.4,
+  // 10.4, 12.4, 13.3; 12.9, 14.4, 17.0, 28.8).
   int parts = 1;
   const long long bytes = (long long)V * (type == VT_FP32 ? 4 : 2);
   while (parts < LP_CLUSTER && rows * parts * 2 <= 148 && bytes / parts >= 48 << 10) parts *= 2;

@@ -73,7 +73,8 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence = QUIN
     is carried with 22 bits up to the last two. Matrices of many different elements come out 0.2 % of the 2-norm off, of which most
     is the result's rounding. Where few numbers repeat (diagonal matrices, permutations, constants, a few elements at all) their
     roundings do not average out: identities are up to 1.2 % off, any one singular value 2.7 % at most. On CPU the products are fp32. A
-    matrix of zeros stays one; NaN or infinity anywhere in a matrix make NaNs of it."""
+    matrix of zeros stays one; NaN or infinity anywhere in a matrix make NaNs of it. There is no derivative on CUDA (on CPU torch records
+    its products)."""
     if g.dim() < 2 or not g.is_floating_point():
         raise ValueError(f"newton_schulz takes floating-point matrices, not {tuple(g.shape)} of {g.dtype}")
     steps = int(steps)
@@ -89,7 +90,6 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence = QUIN
     if m == 0 or n == 0 or count == 0:
         return torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
     if not g.is_cuda:
-        x = g.float()
         norm = g.double().square().sum((-2, -1), keepdim=True).sqrt()
         x = (g.double() / (norm + eps)).float()
         for k in range(steps):

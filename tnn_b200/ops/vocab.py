@@ -89,7 +89,8 @@ def _pitch(t: torch.Tensor) -> int:
 # ------------------------------------------------------------------------------------------------------- embedding
 def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * table[ids]``, shape ``[*ids.shape, width]``: the product in fp32, rounded once to the table's type. Positions
-    whose id is ``padding_idx`` are zero; an id outside the table reads row 0, like :func:`raw.embedding_fwd`."""
+    whose id is ``padding_idx`` are zero; an id outside the table reads row 0, like :func:`raw.embedding_fwd`. No derivative on CUDA:
+    :func:`functional.embedding` has one."""
     if table.dim() != 2 or not table.is_floating_point():
         raise ValueError(f"embedding table {tuple(table.shape)} of {table.dtype}: a floating-point matrix expected")
     rows, width = table.shape
@@ -124,7 +125,9 @@ _FEW = 128  # positions whose gradient is one kernel without workspaces (embeddi
 
 def _chunk(n: int) -> int:
     """Sorted positions per CTA of the gradient's sums: enough CTAs for the SMs (148, several on each), and no more parts of tokens
-    that lie in several chunks than that takes."""
+    that lie in several chunks than that takes. Us of the whole gradient with 16, 32, 64 and 128 (text-like ids): 1000 x 768 bf16 23.0*, 23.0,
+    30.4, 43.4; 8192 x 768 30.0*, 27.6, 33.8, 47.8; 16384 x 1024 48.1*, 43.7, 45.5, 59.6; 20000 x 1001 fp32 65.4, 59.0*, 65.2, 84.9; 50001 x 1001 fp32 109.9, 99.1,
+    104.9*, 105.0; 65536 x 768 bf16 92.8, 78.6, 75.1*, 71.7; 200000 x 768 234.5, 188.7, 170.5, 175.2* (* the one taken)."""
     chunk = 16
     while chunk < 128 and n > 1024 * chunk:
         chunk *= 2
@@ -222,7 +225,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
     Positions of ``ignore_index`` get log probability 0 (their entropy and alternatives are those of their row). Any other token outside
     the vocabulary has log probability NaN. A row with nothing but -inf has log probability -inf and entropy 0; a NaN or +inf logit
     makes a row's results NaN (NaN sorts first, and the indices are those of the largest logits all the same). ``keep``: a dict that
-    receives what :func:`token_log_probs_grad` needs."""
+    receives what :func:`token_log_probs_grad` needs, the entropies of the result among it (which have to stay as they are until then).
+    No derivative on CUDA: :func:`functional.token_log_probs` has one."""
     top_k, temperature, ignore_index, shape = int(top_k), float(temperature), _id(ignore_index), tokens.shape
     V = _check_rows(logits, tokens, top_k, temperature)
     tok = _whole(tokens, logits, "tokens")
