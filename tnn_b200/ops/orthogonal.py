@@ -73,8 +73,8 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Sequence = QUIN
     is carried with 22 bits up to the last two. Matrices of many different elements come out 0.2 % of the 2-norm off, of which most
     is the result's rounding. Where few numbers repeat (diagonal matrices, permutations, constants, a few elements at all) their
     roundings do not average out: with the default coefficients identities are up to 1.2 % off, any one singular value above 1e-4 of the
-    norm 2.7 % at most. On CPU the products are fp32. A matrix of zeros stays one; NaN or infinity anywhere in a matrix make NaNs of it. There is no derivative on CUDA (on CPU torch records
-    its products)."""
+    norm 2.7 % at most. On CPU the products are fp32. A matrix of zeros stays one; NaN or infinity anywhere in a matrix make NaNs of it.
+    There is no derivative on CUDA (on CPU torch records its products)."""
     if g.dim() < 2 or not g.is_floating_point():
         raise ValueError(f"newton_schulz takes floating-point matrices, not {tuple(g.shape)} of {g.dtype}")
     steps = int(steps)
